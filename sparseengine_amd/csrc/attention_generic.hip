@@ -19,7 +19,7 @@ template <typename T>
 __global__ void paged_attention_generic_kernel(
     const T* __restrict__ q, int64_t q_stride, const T* __restrict__ cache,
     const int32_t* __restrict__ block_table, int bt_stride, const int32_t* __restrict__ token_row,
-    const int32_t* __restrict__ positions, T* __restrict__ out, int64_t out_stride, int tokens,
+    const int32_t* __restrict__ positions, T* __restrict__ out, int64_t out_stride, float* __restrict__ lse, int tokens,
     int heads, int kv_heads, int head_dim, int page_size, float scale, int window) {
   extern __shared__ float q_shared[];  // [waves per block][head_dim]
   const int lane = threadIdx.x & (SE_WAVE - 1);
@@ -96,12 +96,13 @@ __global__ void paged_attention_generic_kernel(
     const int d = lane + i * SE_WAVE;
     if (d < head_dim) o[d] = from_float<T>(acc[i] * inv);
   }
+  if (lse != nullptr && lane == 0) lse[static_cast<int64_t>(token) * heads + head] = run_max + logf(run_sum);
 }
 
 extern "C" int se_paged_attention_generic(const void* q, int64_t q_stride, const void* cache,
                                           const int32_t* block_table, int bt_stride,
                                           const int32_t* token_row, const int32_t* positions,
-                                          void* out, int64_t out_stride, int tokens, int heads,
+                                          void* out, int64_t out_stride, float* lse, int tokens, int heads,
                                           int kv_heads, int head_dim, int page_size, float scale,
                                           int window, int dtype, hipStream_t stream) {
   if (tokens <= 0) return SE_OK;
@@ -115,12 +116,12 @@ extern "C" int se_paged_attention_generic(const void* q, int64_t q_stride, const
   if (dtype == SE_F32)
     paged_attention_generic_kernel<float><<<blocks, waves * SE_WAVE, shmem, stream>>>(
         static_cast<const float*>(q), q_stride, static_cast<const float*>(cache), block_table,
-        bt_stride, token_row, positions, static_cast<float*>(out), out_stride, tokens, heads,
+        bt_stride, token_row, positions, static_cast<float*>(out), out_stride, lse, tokens, heads,
         kv_heads, head_dim, page_size, scale, window);
   else
     paged_attention_generic_kernel<bf16_t><<<blocks, waves * SE_WAVE, shmem, stream>>>(
         static_cast<const bf16_t*>(q), q_stride, static_cast<const bf16_t*>(cache), block_table,
-        bt_stride, token_row, positions, static_cast<bf16_t*>(out), out_stride, tokens, heads,
+        bt_stride, token_row, positions, static_cast<bf16_t*>(out), out_stride, lse, tokens, heads,
         kv_heads, head_dim, page_size, scale, window);
   SE_CHECK_LAUNCH();
   return SE_OK;

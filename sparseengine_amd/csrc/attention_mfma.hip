@@ -35,6 +35,11 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 // out), q_start, q_len, ctx_len, slots between two of its tiles (= key ranges per tile), 3 unused
 #define BLOCK_UNIT_FIELDS 12
 
+// The natural logarithm of a row's sum of exponentials from its running maximum (in powers of two) and sum.
+__device__ __forceinline__ float row_logsum(float run_max, float run_sum) {
+  return (run_max + __log2f(run_sum)) * 0.6931471805599453f;
+}
+
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   return static_cast<uint32_t>(float_to_bf16_bits(lo)) |
          (static_cast<uint32_t>(float_to_bf16_bits(hi)) << 16);
@@ -62,7 +67,7 @@ paged_attention_mfma_kernel(const bf16_t* __restrict__ q, int64_t q_stride,
                             const int32_t* __restrict__ block_table, int bt_stride,
                             const int32_t* __restrict__ units, int num_units,
                             bf16_t* __restrict__ out, int64_t out_stride,
-                            float* __restrict__ part_o, float* __restrict__ part_ml, int heads,
+                            float* __restrict__ part_o, float* __restrict__ part_ml, float* __restrict__ lse, int heads,
                             int kv_heads, int page_size, float scale_log2e, int window) {
   constexpr int D = 32 * DSTEPS;
   constexpr int DBLOCKS = 2 * DSTEPS;  // blocks of 16 value dims
@@ -261,6 +266,7 @@ paged_attention_mfma_kernel(const bf16_t* __restrict__ q, int64_t q_stride,
       packed.y = pack_bf16x2(o[db][2] * inv, o[db][3] * inv);
       *reinterpret_cast<uint2*>(o_row + db * 16) = packed;
     }
+    if (lse != nullptr && g == 0) lse[static_cast<int64_t>(token) * heads + head] = row_logsum(run_max, run_sum);
   } else {
     const int64_t base = (static_cast<int64_t>(slot) * kv_heads + kvh) * 16 + n;
     float* po = part_o + base * D + 4 * g;
@@ -381,8 +387,8 @@ paged_attention_tiled_kernel(const bf16_t* __restrict__ q, int64_t q_stride,
                              const int32_t* __restrict__ block_table, int bt_stride,
                              const int32_t* __restrict__ units, bf16_t* __restrict__ out,
                              int64_t out_stride, float* __restrict__ part_o,
-                             float* __restrict__ part_ml, int heads, int kv_heads, int page_size,
-                             float scale_log2e, int window) {
+                             float* __restrict__ part_ml, float* __restrict__ lse, int heads, int kv_heads,
+                             int page_size, float scale_log2e, int window) {
   constexpr int D = 32 * DSTEPS;
   constexpr int DBLOCKS = 2 * DSTEPS;
   constexpr int CHUNKS = 4 * DSTEPS;              // per step: 2 * DSTEPS of keys, then 2 * DSTEPS of values
@@ -863,6 +869,7 @@ paged_attention_tiled_kernel(const bf16_t* __restrict__ q, int64_t q_stride,
       packed.y = pack_bf16x2(o[rt][db][2] * inv, o[rt][db][3] * inv);
       *reinterpret_cast<uint2*>(o_row + db * 16) = packed;
     }
+    if (lse != nullptr && g == 0) lse[static_cast<int64_t>(token) * heads + head] = row_logsum(run_max[rt], total);
   }
 }
 
@@ -874,7 +881,7 @@ paged_attention_tiled_kernel(const bf16_t* __restrict__ q, int64_t q_stride,
 __global__ void __launch_bounds__(256)
 attention_merge_kernel(const int32_t* __restrict__ tasks, const float* __restrict__ part_o,
                        const float* __restrict__ part_ml, bf16_t* __restrict__ out,
-                       int64_t out_stride, int heads, int kv_heads, int head_dim) {
+                       int64_t out_stride, float* __restrict__ lse, int heads, int kv_heads, int head_dim) {
   __shared__ float weight[16][MERGE_MAX_SPLITS];
   __shared__ float inv_denom[16];
   const int32_t* t = tasks + static_cast<int64_t>(blockIdx.x) * TASK_FIELDS;
@@ -904,6 +911,9 @@ attention_merge_kernel(const int32_t* __restrict__ tasks, const float* __restric
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) denom += __shfl_xor(denom, off, SE_WAVE);
     if (j == 0) inv_denom[n] = 1.f / denom;
+    const int rho = row_tile * 16 + n;
+    if (lse != nullptr && j == 0 && rho < q_len * group)
+      lse[static_cast<int64_t>(q_start + rho / group) * heads + kvh * group + rho % group] = row_logsum(m, denom);
   }
   __syncthreads();
   const int vecs_per_row = head_dim / 4;
@@ -939,11 +949,12 @@ attention_merge_kernel(const int32_t* __restrict__ tasks, const float* __restric
   }
 }
 
+// lse: null, or float [tokens, heads] for every row's logarithm of its sum of exponentials.
 extern "C" int se_paged_attention_mfma(const void* q, int64_t q_stride, const void* cache,
                                        const int32_t* block_table, int bt_stride,
                                        const int32_t* units, int num_units, const int32_t* tasks,
                                        int num_tasks, void* out, int64_t out_stride, float* part_o,
-                                       float* part_ml, int heads, int kv_heads, int head_dim,
+                                       float* part_ml, float* lse, int heads, int kv_heads, int head_dim,
                                        int page_size, float scale, int window, hipStream_t stream) {
   if (num_units <= 0 && num_tasks <= 0) return SE_OK;
   if (head_dim % 32 || head_dim <= 0 || head_dim > 256) return SE_ERR_SHAPE;
@@ -958,7 +969,7 @@ extern "C" int se_paged_attention_mfma(const void* q, int64_t q_stride, const vo
     paged_attention_mfma_kernel<DS><<<grid, 256, 0, stream>>>(                                     \
         static_cast<const bf16_t*>(q), q_stride, static_cast<const bf16_t*>(cache), block_table,  \
         bt_stride, units, num_units, static_cast<bf16_t*>(out), out_stride,                       \
-        part_o, part_ml, heads, kv_heads, page_size, scale_log2e, window);                        \
+        part_o, part_ml, lse, heads, kv_heads, page_size, scale_log2e, window);                   \
     break;
   switch (head_dim / 32) {
     SE_ATT(1) SE_ATT(2) SE_ATT(3) SE_ATT(4) SE_ATT(5) SE_ATT(6) SE_ATT(7) SE_ATT(8)
@@ -969,7 +980,7 @@ extern "C" int se_paged_attention_mfma(const void* q, int64_t q_stride, const vo
   }
   if (num_tasks > 0) {   // also merges what the block kernel has left in the same buffers
     attention_merge_kernel<<<dim3(num_tasks, kv_heads), 256, 0, stream>>>(
-        tasks, part_o, part_ml, static_cast<bf16_t*>(out), out_stride, heads,
+        tasks, part_o, part_ml, static_cast<bf16_t*>(out), out_stride, lse, heads,
         kv_heads, head_dim);
     SE_CHECK_LAUNCH();
   }
@@ -982,7 +993,7 @@ extern "C" int se_paged_attention_mfma(const void* q, int64_t q_stride, const vo
 extern "C" int se_paged_attention_tiled(const void* q, int64_t q_stride, const void* cache,
                                         const int32_t* block_table, int bt_stride,
                                         const int32_t* units, int num_units, void* out,
-                                        int64_t out_stride, float* part_o, float* part_ml, int heads,
+                                        int64_t out_stride, float* part_o, float* part_ml, float* lse, int heads,
                                         int kv_heads, int head_dim, int page_size, float scale,
                                         int window, int tiles_per_block, hipStream_t stream) {
   if (num_units <= 0) return SE_OK;
@@ -1007,7 +1018,7 @@ extern "C" int se_paged_attention_tiled(const void* q, int64_t q_stride, const v
     }                                                                                              \
     paged_attention_tiled_kernel<DS, TILED_ROW_TILES, TILED_STAGES, IN_PAGE><<<grid, 256, shared, stream>>>( \
         static_cast<const bf16_t*>(q), q_stride, static_cast<const bf16_t*>(cache), block_table,  \
-        bt_stride, units, static_cast<bf16_t*>(out), out_stride, part_o, part_ml, heads,          \
+        bt_stride, units, static_cast<bf16_t*>(out), out_stride, part_o, part_ml, lse, heads,     \
         kv_heads, page_size, scale_log2e, window);                                                 \
   }
 #define SE_ATT(DS)                                                                                 \

@@ -113,6 +113,14 @@ def build_attention_work(q_len, ctx_len, group: int, kv_heads: int, window: int 
     return AttentionWork(units, tasks, int(counts[3]), blocks)
 
 
+def items_in_blocks(q_len, group: int, head_dim: int) -> np.ndarray:
+    """Which items go to the block kernel: those with at least half a block of tiles."""
+    tiles = (np.asarray(q_len, dtype=np.int64) * group + 15) // 16
+    if not head_dim or head_dim % 32 or head_dim > TILED_MAX_HEAD_DIM:
+        return np.zeros(tiles.size, dtype=bool)
+    return tiles >= TILES_PER_BLOCK // 2
+
+
 def build_attention_work_numpy(q_len, ctx_len, group: int, kv_heads: int, window: int = 0,
                                target_waves: int = TARGET_WAVES, head_dim: int = 0) -> AttentionWork:
     """``head_dim``: 0 keeps every item on the one-wavefront kernel (callers that do not know it).
@@ -128,9 +136,7 @@ def build_attention_work_numpy(q_len, ctx_len, group: int, kv_heads: int, window
     q_start = np.concatenate(([0], np.cumsum(q_len)[:-1]))      # items' tokens lie one after the other
     tiles = (q_len * group + 15) // 16
     reach = np.minimum(ctx_len, window + q_len) if window else ctx_len      # keys an item's tiles can read
-    in_blocks = np.zeros(len(tiles), dtype=bool)
-    if head_dim and head_dim % 32 == 0 and head_dim <= TILED_MAX_HEAD_DIM:
-        in_blocks = tiles >= TILES_PER_BLOCK // 2
+    in_blocks = items_in_blocks(q_len, group, head_dim)
 
     def keys_per_unit(units_per_item, wanted: int, least: int) -> int:
         """Keys of a range so that all ranges together number about ``wanted``."""

@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 from ctypes import c_float, c_int, c_int64, c_void_p
 
+import numpy as np
 import torch
 
 from . import library
@@ -56,6 +57,14 @@ def _require(cond: bool, message: str):
         raise ValueError(message)
 
 
+def _same_device(*tensors):
+    """All on one device, and that the current one: a launch goes to the current device's current stream."""
+    device = tensors[0].device
+    _require(all(t is None or t.device == device for t in tensors), "the tensors of a call must be on one device")
+    _require(device.type != "cuda" or device.index == torch.cuda.current_device(),
+             "the tensors of a call must be on the current device")
+
+
 def _i32(t: torch.Tensor, name: str):
     _require(t.dtype == torch.int32 and t.is_contiguous(), f"{name} must be contiguous int32")
 
@@ -75,20 +84,44 @@ _SIGNATURES = {
     },
     "attention_generic": {
         "se_paged_attention_generic": [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p,
-                                       c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int,
+                                       c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int,
                                        c_int, c_float, c_int, c_int, c_void_p],
     },
     "attention_mfma": {
         # q, q_stride, cache, block_table, bt_stride, units, num_units, tasks, num_tasks, out, out_stride,
-        # part_o, part_ml, heads, kv_heads, head_dim, page_size, scale, window, stream
+        # part_o, part_ml, lse, heads, kv_heads, head_dim, page_size, scale, window, stream
         "se_paged_attention_mfma": [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p,
-                                    c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                                    c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                     c_float, c_int, c_void_p],
         # q, q_stride, cache, block_table, bt_stride, units, num_units, out, out_stride, part_o, part_ml,
-        # heads, kv_heads, head_dim, page_size, scale, window, tiles_per_block, stream
+        # lse, heads, kv_heads, head_dim, page_size, scale, window, tiles_per_block, stream
         "se_paged_attention_tiled": [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p,
-                                     c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int,
+                                     c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int,
                                      c_int, c_void_p],
+    },
+    "attention_fp4": {
+        # q, q_stride, cache, block_table, bt_stride, units, num_units, out, out_stride, part_o, part_ml, lse,
+        # heads, kv_heads, head_dim, page_size, scale, window, stream
+        "se_paged_attention_fp4": [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64,
+                                   c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p],
+    },
+    "cache_fp4": {
+        # qkv, row_stride, slots, tokens, heads, kv_heads, head_dim, cache, page_size, dtype, stream
+        "se_fp4_store": [c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p],
+        # cache, pages, bt_stride, list, count, out, kv_heads, page_size, head_dim, dtype, stream
+        "se_fp4_unpack": [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
+    },
+    "attention_weights": {
+        # q, q_stride, cache, kind, block_table, bt_stride, item_meta, items, longest, lse, previous, out, heads,
+        # kv_heads, head_dim, page_size, scale, window, dtype, stream
+        "se_attention_weights": [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p,
+                                 c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
+    },
+    "evict": {
+        # cache, kind, weights, block_table, bt_stride, lengths, items, longest, new_table, new_stride, keep, recent,
+        # kept, kv_heads, page_size, head_dim, stream
+        "se_evict_tokens": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int, c_int,
+                            c_int, c_void_p, c_int, c_int, c_int, c_void_p],
     },
     "moe": {
         "se_router_topk": [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
@@ -192,7 +225,7 @@ class HipKernels:
     """The kernel interface of the engine, served by the gfx950 libraries."""
 
     libraries = ("norm", "rope_kv", "attention_generic", "attention_mfma", "moe", "moe_mfma", "sampling",
-                 "host_work", "memory_probe")
+                 "host_work", "memory_probe", "cache_fp4", "attention_fp4", "attention_weights", "evict")
 
     def __init__(self):
         if not torch.cuda.is_available():
@@ -321,10 +354,15 @@ class HipKernels:
         ``per_head_norm``, one statistic per token and head, weights ``[head_dim]``), partial rotation by
         ``cos_sin [max_pos, rotary_dim]`` (cos half, sin half; ``pairing`` "neox" turns dims ``(d, d + rotary_dim / 2)`` together, "interleaved" dims ``(2 j, 2 j + 1)``), and
         the write of k and v to ``cache [pages, 2, kv_heads, page_size, head_dim]`` at ``slots`` (the
-        last two sizes are a page's geometry; the order of its elements is cache/layout.py's)."""
+        last two sizes are a page's geometry; the order of its elements is cache/layout.py's).  A uint8 cache
+        ``[pages, 2, kv_heads, page_size, head_dim * 17 / 32]`` takes the stored (rounded) k and v in 4 bits
+        (cache/layout.py; head sizes and pages in steps of 32).  Slots below 0 are skipped."""
         tokens = qkv.shape[0]
         width = (heads + 2 * kv_heads) * head_dim
         int32 = torch.int32
+        if cache is not None and cache.dtype == torch.uint8:
+            return self._store_fp4(qkv, positions, cos_sin, q_weight, k_weight, eps, heads, kv_heads, head_dim,
+                                   rotary_dim, cache, slots, page_size, pairing, per_head_norm)
         # the call of every layer (norm weights, a rotation table, the cache write) in one expression; a call that
         # fails a check, and every other kind of call, takes the long way below, which names what is wrong
         if (_SHORT_WAYS and not per_head_norm and q_weight is not None and cache is not None and rotary_dim
@@ -378,7 +416,203 @@ class HipKernels:
             self.ROTARY_PAIRINGS[pairing], int(bool(per_head_norm and q_weight is not None)), _stream()),
             "qk_norm_rope_store")
 
-    def paged_attention(self, q, cache, meta, out, scale: float, window: int = 0):
+    # ------------------------------------------------------------------ the cache in 4 bits
+    def _fp4_cache(self, cache, head_dim: int, page_size: int | None = None):
+        """Checks a 4-bit cache layer; its page size."""
+        _require(cache.dim() == 5 and cache.shape[1] == 2 and cache.is_contiguous() and cache.dtype == torch.uint8
+                 and cache.shape[4] * 32 == head_dim * 17, "4-bit cache layout")
+        page = cache.shape[3]
+        _require(page_size is None or page == page_size, "4-bit cache: page size")
+        if head_dim % 32 or head_dim > 512 or page % 32:
+            raise KernelShapeError(f"a 4-bit cache takes head sizes in steps of 32 up to 512 and pages in steps of 32 "
+                                   f"tokens, got head_dim {head_dim} and page_size {page}")
+        if cache.data_ptr() % 16:
+            raise KernelShapeError("a 4-bit cache has to begin on a multiple of 16 bytes")
+        return page
+
+    def _store_fp4(self, qkv, positions, cos_sin, q_weight, k_weight, eps, heads, kv_heads, head_dim, rotary_dim, cache,
+                   slots, page_size, pairing, per_head_norm):
+        tokens = qkv.shape[0]
+        self._fp4_cache(cache, head_dim, page_size)
+        _require(cache.shape[2] == kv_heads, "4-bit cache layout")
+        _i32(slots, "slots")
+        _require(slots.numel() == tokens, "slots length")
+        _require(qkv.dim() == 2 and qkv.shape[1] == (heads + 2 * kv_heads) * head_dim and qkv.stride(1) == 1, "qkv shape")
+        _same_device(qkv, cache, slots)
+        if qkv.stride(0) % 8 or qkv.data_ptr() % 16:
+            raise KernelShapeError("4-bit cache write: qkv rows have to begin on multiples of 16 bytes")
+        if q_weight is not None or rotary_dim:
+            self.qk_norm_rope_store(qkv, positions, cos_sin, q_weight, k_weight, eps, heads, kv_heads, head_dim,
+                                    rotary_dim, None, None, page_size, pairing=pairing, per_head_norm=per_head_norm)
+        _check(_fn.get("cache_fp4", "se_fp4_store")(
+            _ptr(qkv), qkv.stride(0), _ptr(slots), tokens, heads, kv_heads, head_dim, _ptr(cache), page_size,
+            _code(qkv.dtype), _stream()), "qk_norm_rope_store (4-bit cache)")
+
+    def unpack_cache(self, cache, pages, out):
+        """Page ``pages[i]`` (int32; below 0: left out) of a 4-bit cache layer to page ``i`` of ``out [n, 2, kv_heads,
+        page_size, head_dim]``, in the order of the engine's own cache (cache/layout.py) and in ``out``'s type."""
+        _i32(pages, "pages")
+        _require(out.dim() == 5 and out.is_contiguous() and out.shape[0] == pages.numel() and out.shape[1:4] == cache.shape[1:4],
+                 "unpack_cache: out [pages, 2, kv_heads, page_size, head_dim]")
+        page = self._fp4_cache(cache, out.shape[4])
+        _same_device(cache, pages, out)
+        if out.data_ptr() % 16:
+            raise KernelShapeError("unpack_cache: out has to begin on a multiple of 16 bytes")
+        _check(_fn.get("cache_fp4", "se_fp4_unpack")(
+            _ptr(cache), _ptr(pages), 0, None, pages.numel(), _ptr(out), cache.shape[2], page, out.shape[4],
+            _code(out.dtype), _stream()), "unpack_cache")
+
+    FP4_HEAD_DIMS = (64, 128, 256)      # head sizes that the 4-bit attention kernel is built for
+
+    def _paged_attention_fp4(self, q, cache, meta, out, scale, window, lse):
+        """Attention over a 4-bit cache.  In bfloat16, at the head sizes its kernel takes, items of few rows (the
+        work list's units) are read in 4 bits; the pages of items of many rows (its blocks: a page is then read
+        once per block of rows, and turning it into bfloat16 each time would cost more than the products), and of
+        everything else, are unpacked to a temporary cache in the engine's own layout first."""
+        tokens, heads, head_dim = q.shape
+        page = self._fp4_cache(cache, head_dim)
+        kv_heads = cache.shape[2]
+        if getattr(meta, "item_q_len", None) is None:
+            raise ValueError("attention over a 4-bit cache needs the step's items (item_q_len, item_ctx_len)")
+        _require(scale > 0, "attention over a 4-bit cache: scale must be positive")
+        direct = q.dtype == torch.bfloat16 and head_dim in self.FP4_HEAD_DIMS
+        group = heads // kv_heads
+        work = self._attention_work(q, meta, heads, kv_heads, head_dim, window) if q.dtype == torch.bfloat16 else None
+        unpack = None
+        if not direct or work.num_block_units:
+            unpack = self._fp4_unpack_list(meta, group, head_dim, page, window, only_blocks=direct)
+        scratch = scratch_table = None
+        if unpack is not None:
+            pairs, scratch_table = unpack
+            scratch = torch.empty(pairs.shape[0], 2, kv_heads, page, head_dim, dtype=q.dtype, device=q.device)
+            _check(_fn.get("cache_fp4", "se_fp4_unpack")(
+                _ptr(cache), _ptr(meta.block_table), meta.block_table.stride(0), _ptr(pairs), pairs.shape[0], _ptr(scratch),
+                kv_heads, page, head_dim, _code(q.dtype), _stream()), "paged_attention (unpacking 4-bit pages)")
+        if not direct:
+            if q.dtype == torch.bfloat16 and head_dim <= 256:
+                self._run_attention_work(q, scratch, scratch_table, work, out, scale, window, lse)
+            else:
+                self._paged_attention_generic(q, scratch, scratch_table, meta, out, scale, window, lse)
+            return
+        self._run_attention_work(q, scratch, scratch_table, work, out, scale, window, lse, fp4=(cache, meta.block_table))
+
+    def _fp4_unpack_list(self, meta, group: int, head_dim: int, page: int, window: int, only_blocks: bool):
+        """(int32 ``[n, 2]`` block-table places to unpack, int32 ``[items, columns]`` where each lies among them), on
+        the device; made once per step and kept with the step's work lists."""
+        kept = getattr(meta, "work", None)
+        key = ("unpack", group, head_dim, page, window, only_blocks)
+        if kept is not None and key in kept:
+            return kept[key]
+        from .attention_work import items_in_blocks
+        q_len, ctx_len = np.asarray(meta.item_q_len, dtype=np.int64), np.asarray(meta.item_ctx_len, dtype=np.int64)
+        chosen = items_in_blocks(q_len, group, head_dim) if only_blocks else np.ones(q_len.size, dtype=bool)
+        low = np.maximum(0, ctx_len - q_len - window + 1) if window else np.zeros_like(ctx_len)
+        first, until = low // page, -(-ctx_len // page)
+        column = np.arange(int(until.max()))[None, :]
+        read = (column >= first[:, None]) & (column < until[:, None]) & chosen[:, None]
+        pairs = np.ascontiguousarray(np.argwhere(read), dtype=np.int32)
+        table = np.zeros(read.shape, dtype=np.int32)
+        table[read] = np.arange(pairs.shape[0], dtype=np.int32)
+        device = meta.block_table.device
+        made = (torch.from_numpy(pairs).to(device), torch.from_numpy(table).to(device))
+        if kept is not None:
+            kept[key] = made
+        return made
+
+    # ------------------------------------------------------------------ letting tokens go
+    _CACHE_KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.uint8: 2}
+
+    def attention_weights(self, q, cache, meta, lse, out, scale: float, window: int = 0, previous=None):
+        """The softmax weight that every cached key gets from the step's rows, per kv head (summed over the kv
+        head's query heads and the step's tokens): ``out[key] = previous[key] + sum exp(scale q . k - lse)``.
+
+        ``q``, ``cache``, ``meta``, ``scale`` and ``window`` as in ``paged_attention``, whose ``lse [T, heads]`` (float32)
+        goes in here; ``meta`` needs its items.  ``out`` and ``previous``: float32 ``[pages, kv_heads, page_size]`` in
+        the cache's pages; they may be the same tensor.  ``previous`` counts for the keys that are older than the
+        step (None: nothing for them either); the step's own keys begin with 0.  Keys that no row can see (a window)
+        are left as they are."""
+        tokens, heads, head_dim = q.shape
+        fp4 = cache.dtype == torch.uint8
+        _require(q.stride(2) == 1 and q.stride(1) == head_dim, "q heads must be dense")
+        if fp4:
+            self._fp4_cache(cache, head_dim)
+        else:
+            _require(cache.dim() == 5 and cache.shape[1] == 2 and cache.shape[4] == head_dim and cache.is_contiguous()
+                     and cache.dtype == q.dtype, "cache layout")
+        pages, _, kv_heads, page = cache.shape[:4]
+        _code(q.dtype)
+        if heads % kv_heads:
+            raise KernelShapeError(f"attention weights: {heads} heads do not divide into {kv_heads} kv heads")
+        if page % 8 or head_dim % 8 or head_dim > 512 or q.stride(0) % 8 or q.data_ptr() % 16:
+            raise KernelShapeError(f"attention weights: page_size {page} and head_dim {head_dim} in steps of 8 (head_dim "
+                                   "at most 512), q rows on multiples of 16 bytes")
+        for name, w in (("out", out), ("previous", previous)):
+            _require(w is None or (w.dtype == torch.float32 and w.is_contiguous() and tuple(w.shape) == (pages, kv_heads, page)),
+                     f"attention weights: {name} must be contiguous float32 [pages, kv_heads, page_size]")
+        _require(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (tokens, heads),
+                 "attention weights: lse must be contiguous float32 [tokens, heads]")
+        _require(meta.block_table.dtype == torch.int32 and meta.block_table.dim() == 2 and meta.block_table.stride(1) == 1,
+                 "block_table layout")
+        items, longest, item_meta = self._items(meta, tokens, page)
+        _same_device(q, cache, lse, out, previous, meta.block_table, item_meta)
+        _check(_fn.get("attention_weights", "se_attention_weights")(
+            _ptr(q), q.stride(0), _ptr(cache), self._CACHE_KINDS[cache.dtype], _ptr(meta.block_table),
+            meta.block_table.stride(0), _ptr(item_meta), items, longest, _ptr(lse), _ptr(previous), _ptr(out), heads, kv_heads,
+            head_dim, page, float(scale), int(window or 0), _code(q.dtype), _stream()), "attention_weights")
+
+    def _items(self, meta, tokens: int, page: int):
+        """(number of items, longest context, int32 ``[3, items]`` on the device) of a step, checked."""
+        if getattr(meta, "item_q_len", None) is None:
+            raise ValueError("attention weights need the step's items (item_q_len, item_ctx_len)")
+        q_len, ctx_len = np.asarray(meta.item_q_len), np.asarray(meta.item_ctx_len)
+        _require(q_len.size == ctx_len.size and q_len.size <= meta.block_table.shape[0] and bool((q_len >= 1).all())
+                 and bool((q_len <= ctx_len).all()) and int(q_len.sum()) == tokens,
+                 "items: every item needs at least one new token and no more than its context, together the step's tokens")
+        longest = int(ctx_len.max())
+        _require(longest <= meta.block_table.shape[1] * page, "the block table has too few columns for the longest item")
+        item_meta = getattr(meta, "item_meta", None)
+        if item_meta is None:
+            start = np.concatenate(([0], np.cumsum(q_len)[:-1]))
+            item_meta = torch.from_numpy(np.stack([start, q_len, ctx_len]).astype(np.int32)).to(meta.block_table.device)
+        _require(item_meta.dtype == torch.int32 and item_meta.is_contiguous() and tuple(item_meta.shape) == (3, q_len.size),
+                 "item_meta must be contiguous int32 [3, items]")
+        return q_len.size, longest, item_meta
+
+    def evict_tokens(self, cache, weights, block_table, lengths, new_table, keep: int, recent: int, kept, longest: int):
+        """Of every request's ``lengths[i]`` cached tokens (int32; at most ``longest``) and of every kv head apart, the
+        last ``recent`` and the heaviest others by ``weights`` (float32 ``[pages, kv_heads, page_size]``; ties: the
+        first), ``keep`` in all, are copied in their order to the pages of ``new_table`` (int32 ``[items,
+        ceil(keep / page_size)]``), with their weights.  ``kept`` (int32 ``[items, kv_heads, keep]``) receives their
+        old places, ascending, -1 behind the last where a request has fewer.  ``cache`` is a layer in float32,
+        bfloat16 or 4 bits.  The new pages must be none of the requests' old ones and no two the same; the old
+        pages stay as they are.  Rows of ``new_table`` with entries below 0 are filled up to those."""
+        fp4 = cache.dtype == torch.uint8
+        _require(cache.dim() == 5 and cache.shape[1] == 2 and cache.is_contiguous() and cache.dtype in self._CACHE_KINDS,
+                 "cache layout")
+        pages, _, kv_heads, page, row = cache.shape
+        head_dim = row * 32 // 17 if fp4 else row
+        if fp4:
+            self._fp4_cache(cache, head_dim)
+        if page % 8 or head_dim % 8 or page > 4096 or cache.data_ptr() % 16:
+            raise KernelShapeError(f"eviction: page_size {page} and head_dim {head_dim} in steps of 8, pages of at most 4096 tokens")
+        keep, recent, longest = int(keep), int(recent), int(longest)
+        _require(keep >= 1 and 0 <= recent <= keep, "eviction: 1 <= keep, 0 <= recent <= keep")
+        _require(weights.dtype == torch.float32 and weights.is_contiguous() and tuple(weights.shape) == (pages, kv_heads, page),
+                 "eviction: weights must be contiguous float32 [pages, kv_heads, page_size]")
+        _i32(lengths, "lengths")
+        items = lengths.numel()
+        for name, table, columns in (("block_table", block_table, -(-longest // page)), ("new_table", new_table, -(-keep // page))):
+            _require(table.dtype == torch.int32 and table.dim() == 2 and table.stride(1) == 1 and table.shape[0] == items
+                     and table.shape[1] >= columns, f"eviction: {name} must be int32 [items, at least {columns}]")
+        _i32(kept, "kept")
+        _require(tuple(kept.shape) == (items, kv_heads, keep), "eviction: kept must be int32 [items, kv_heads, keep]")
+        _same_device(cache, weights, block_table, lengths, new_table, kept)
+        _check(_fn.get("evict", "se_evict_tokens")(
+            _ptr(cache), self._CACHE_KINDS[cache.dtype], _ptr(weights), _ptr(block_table), block_table.stride(0), _ptr(lengths),
+            items, longest, _ptr(new_table), new_table.stride(0), keep, recent, _ptr(kept), kv_heads, page, head_dim, _stream()),
+            "evict_tokens")
+
+    def paged_attention(self, q, cache, meta, out, scale: float, window: int = 0, lse=None):
         """Causal attention of every token of the step against its request's pages.
 
         ``q``: ``[T, heads, head_dim]`` view (token stride free, heads dense); ``cache``:
@@ -386,12 +620,19 @@ class HipKernels:
         (int32 ``[items, max_pages]``), ``token_row`` and ``positions`` (int32 ``[T]``) and, for the
         matrix-core kernels, the items' lengths on the host (``item_q_len``, ``item_ctx_len``) and
         optionally prepared work lists (``work``);
-        ``out``: ``[T, heads * head_dim]``."""
+        ``out``: ``[T, heads * head_dim]``; ``lse``: None, or float32 ``[T, heads]`` that receives every row's
+        logarithm of its sum of exponentials.  A uint8 ``cache`` holds keys and values in 4 bits (``[pages, 2, kv_heads,
+        page_size, head_dim * 17 / 32]``, cache/layout.py): ``meta`` then needs its items, ``scale`` is positive, and
+        the call allocates what its longer way needs."""
         tokens, heads, head_dim = q.shape
         kv_heads, page_size = cache.shape[2], cache.shape[3]
         _require(q.stride(2) == 1 and q.stride(1) == head_dim, "q heads must be dense")
-        _require(cache.dim() == 5 and cache.shape[1] == 2 and cache.shape[4] == head_dim
-                 and cache.is_contiguous() and cache.dtype == q.dtype, "cache layout")
+        fp4 = cache.dtype == torch.uint8
+        _require(fp4 or (cache.dim() == 5 and cache.shape[1] == 2 and cache.shape[4] == head_dim
+                         and cache.is_contiguous() and cache.dtype == q.dtype), "cache layout")
+        if lse is not None:
+            _require(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (tokens, heads),
+                     "attention: lse must be contiguous float32 [tokens, heads]")
         _require(out.shape == (tokens, heads * head_dim) and out.stride(1) == 1 and out.dtype == q.dtype,
                  "attention out shape")
         _i32(meta.token_row, "token_row"); _i32(meta.positions, "positions")
@@ -403,24 +644,33 @@ class HipKernels:
         if page_size % 8:
             raise KernelShapeError(f"attention: page_size {page_size} must be a multiple of 8")
         window = int(window or 0)
+        if fp4:
+            _same_device(q, cache, out, lse, meta.block_table)
+            if q.stride(0) % 8 or out.stride(0) % 8 or q.data_ptr() % 16 or out.data_ptr() % 16:
+                raise KernelShapeError("attention over a 4-bit cache: rows of q and out have to begin on multiples of 16 bytes")
+            return self._paged_attention_fp4(q, cache, meta, out, float(scale), window, lse)
         if (q.dtype == torch.bfloat16 and head_dim % 32 == 0 and head_dim <= 256
                 and getattr(meta, "item_q_len", None) is not None):      # the step's items are known
-            return self._paged_attention_mfma(q, cache, meta, out, scale, window)
+            work = self._attention_work(q, meta, heads, kv_heads, head_dim, window)
+            return self._run_attention_work(q, cache, meta.block_table, work, out, scale, window, lse)
+        self._paged_attention_generic(q, cache, meta.block_table, meta, out, scale, window, lse)
+
+    def _paged_attention_generic(self, q, cache, block_table, meta, out, scale, window, lse):
+        tokens, heads, head_dim = q.shape
+        kv_heads, page_size = cache.shape[2], cache.shape[3]
         if head_dim % 8 or head_dim > 512:
             raise KernelShapeError(f"attention: head_dim {head_dim} must be a multiple of 8, at most 512")
         _check(_fn.get("attention_generic", "se_paged_attention_generic")(
-            _ptr(q), q.stride(0), _ptr(cache), _ptr(meta.block_table), meta.block_table.stride(0),
-            _ptr(meta.token_row), _ptr(meta.positions), _ptr(out), out.stride(0), tokens, heads,
+            _ptr(q), q.stride(0), _ptr(cache), _ptr(block_table), block_table.stride(0),
+            _ptr(meta.token_row), _ptr(meta.positions), _ptr(out), out.stride(0), _ptr(lse), tokens, heads,
             kv_heads, head_dim, page_size, float(scale), window, _code(q.dtype), _stream()),
             "paged_attention")
 
-    def _paged_attention_mfma(self, q, cache, meta, out, scale, window):
-        """Matrix-core path: work units (row tile x key range) from the step's item lengths."""
-        tokens, heads, head_dim = q.shape
-        kv_heads, page_size = cache.shape[2], cache.shape[3]
+    def _attention_work(self, q, meta, heads, kv_heads, head_dim, window):
+        """The step's work lists of the matrix-core kernels, prepared by the batch builder or built here."""
         group = heads // kv_heads
         work = None if getattr(meta, "work", None) is None else meta.work.get((group, window))
-        if work is None:                      # not prepared by the batch builder: build it here
+        if work is None:
             from .attention_work import DeviceAttentionWork, build_attention_work
             host = build_attention_work(meta.item_q_len, meta.item_ctx_len, group, kv_heads, window,
                                         head_dim=head_dim)
@@ -430,29 +680,48 @@ class HipKernels:
                 torch.from_numpy(host.block_units).to(q.device), host.block_units.shape[0], host.tiles_per_block)
             if getattr(meta, "work", None) is not None:
                 meta.work[(group, window)] = work
+        return work
+
+    def _run_attention_work(self, q, cache, block_table, work, out, scale, window, lse, fp4=None):
+        """Matrix-core path: work units (row tile x key range) from the step's item lengths.  ``fp4``: None, or
+        (4-bit cache, its block table) that the single-wavefront units read; ``cache`` is then what the blocks read."""
+        tokens, heads, head_dim = q.shape
+        kv_heads, page_size = (cache if fp4 is None else fp4[0]).shape[2:4]
         part_o = part_ml = None
         if work.num_slots:                    # key ranges leave partial results for the merge
             need = work.num_slots * kv_heads * 16
-            if self._attention_partials is None or self._attention_partials[0].numel() < need * head_dim:
-                self._attention_partials = (torch.empty(need * head_dim, dtype=torch.float32, device=q.device),
-                                            torch.empty(need * 2, dtype=torch.float32, device=q.device))
-            part_o, part_ml = self._attention_partials
-            if part_ml.numel() < need * 2:
+            if fp4 is not None:               # the call's own: nothing of another stream's or graph's is reused
+                part_o = torch.empty(need * head_dim, dtype=torch.float32, device=q.device)
                 part_ml = torch.empty(need * 2, dtype=torch.float32, device=q.device)
-                self._attention_partials = (part_o, part_ml)
+            else:
+                if self._attention_partials is None or self._attention_partials[0].numel() < need * head_dim:
+                    self._attention_partials = (torch.empty(need * head_dim, dtype=torch.float32, device=q.device),
+                                                torch.empty(need * 2, dtype=torch.float32, device=q.device))
+                part_o, part_ml = self._attention_partials
+                if part_ml.numel() < need * 2:
+                    part_ml = torch.empty(need * 2, dtype=torch.float32, device=q.device)
+                    self._attention_partials = (part_o, part_ml)
         if work.num_block_units:              # prompt portions: keys and values shared by a block
             _check(_fn.get("attention_mfma", "se_paged_attention_tiled")(
-                _ptr(q), q.stride(0), _ptr(cache), _ptr(meta.block_table), meta.block_table.stride(0),
+                _ptr(q), q.stride(0), _ptr(cache), _ptr(block_table), block_table.stride(0),
                 _ptr(work.block_units), work.num_block_units, _ptr(out), out.stride(0), _ptr(part_o),
-                _ptr(part_ml), heads, kv_heads, head_dim, page_size, float(scale), window,
+                _ptr(part_ml), _ptr(lse), heads, kv_heads, head_dim, page_size, float(scale), window,
                 work.tiles_per_block, _stream()), "paged_attention (blocks)",
                 "head_dim a multiple of 32 up to 128, page_size a multiple of 8")
-        if work.num_units or work.num_tasks:  # one wavefront per tile and key range; then all merges
+        units = work.num_units
+        if fp4 is not None and units:
+            fp4_cache, fp4_table = fp4
+            _check(_fn.get("attention_fp4", "se_paged_attention_fp4")(
+                _ptr(q), q.stride(0), _ptr(fp4_cache), _ptr(fp4_table), fp4_table.stride(0), _ptr(work.units), units,
+                _ptr(out), out.stride(0), _ptr(part_o), _ptr(part_ml), _ptr(lse), heads, kv_heads, head_dim, page_size,
+                float(scale), window, _stream()), "paged_attention (4-bit cache)", "head_dim 64, 128 or 256")
+            units = 0                         # what is left for the call below: the merges
+        if units or work.num_tasks:           # one wavefront per tile and key range; then all merges
             _check(_fn.get("attention_mfma", "se_paged_attention_mfma")(
-                _ptr(q), q.stride(0), _ptr(cache), _ptr(meta.block_table), meta.block_table.stride(0),
-                _ptr(work.units) if work.num_units else None, work.num_units,
+                _ptr(q), q.stride(0), _ptr(cache), _ptr(block_table), 0 if block_table is None else block_table.stride(0),
+                _ptr(work.units) if units else None, units,
                 _ptr(work.tasks) if work.num_tasks else None, work.num_tasks, _ptr(out), out.stride(0),
-                _ptr(part_o), _ptr(part_ml), heads, kv_heads, head_dim, page_size, float(scale), window,
+                _ptr(part_o), _ptr(part_ml), _ptr(lse), heads, kv_heads, head_dim, page_size, float(scale), window,
                 _stream()), "paged_attention (wavefronts)",
                 "head_dim a multiple of 32 up to 256, page_size a multiple of 8")
 

@@ -32,6 +32,7 @@ HIPCC_FLAGS = [
 # in every step of the key loop, which costs more instructions than the step's own arithmetic.
 EXTRA_FLAGS = {
     "attention_mfma": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "attention_fp4": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -19,7 +19,8 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 CSRC = HERE.parent.parent / "sparseengine_amd" / "csrc"
-SOURCES = ("norm", "rope_kv", "attention_generic", "attention_mfma", "moe", "moe_mfma", "sampling")
+SOURCES = ("norm", "rope_kv", "attention_generic", "attention_mfma", "moe", "moe_mfma", "sampling", "cache_fp4",
+           "attention_fp4", "attention_weights", "evict")
 FLAGS = ["-O2", "-g", "-std=c++17", "-shared", "-fPIC", "-x", "c++", "-Wno-unknown-pragmas", "-Wno-pass-failed",
          "-Wno-unused-value", "-Wno-gnu-designator", "-fno-strict-aliasing"]
 

@@ -528,16 +528,42 @@ inline void emu_s_waitcnt(int imm) {
   emu_complete_lds(emu.current, vmcnt);
 }
 
+// v_cvt_scalef32_pk_bf16_fp4: byte `which` of `word` holds two e2m1 codes, the lower first; the factor's exponent
+// field is all that is taken of it (255: not a number)
+inline uint32_t emu_fp4_pair(uint32_t word, float factor, int which) {
+  static const float levels[8] = {0.f, 0.5f, 1.f, 1.5f, 2.f, 3.f, 4.f, 6.f};
+  const int exponent = static_cast<int>(__float_as_uint(factor) >> 23 & 255u);
+  uint32_t out = 0;
+  for (int half = 0; half < 2; ++half) {
+    const uint32_t code = word >> (8 * which + 4 * half) & 15u;
+    const double size = exponent == 255 ? std::nan("") : std::ldexp(static_cast<double>(levels[code & 7u]), exponent - 127);
+    // exact as a bfloat16 (or infinite)
+    const uint32_t bits = exponent == 255 ? 0x7fc00000u : __float_as_uint(static_cast<float>(size)) | (code & 8u) << 28;
+    out |= (bits >> 16) << (16 * half);
+  }
+  return out;
+}
+// v_perm_b32: byte i of the result is byte sel[i] of (b, a), b's bytes first (0 to 3)
+inline uint32_t emu_perm(uint32_t a, uint32_t b, uint32_t sel) {
+  const uint64_t both = static_cast<uint64_t>(a) << 32 | b;
+  uint32_t out = 0;
+  for (int i = 0; i < 4; ++i) out |= static_cast<uint32_t>(both >> (8 * (sel >> (8 * i) & 7u)) & 255u) << (8 * i);
+  return out;
+}
+
 inline float emu_max_bare(float a, float b) { return fmaxf(a, b); }
 inline float emu_max3_bare(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
 #define __builtin_amdgcn_mfma_f32_16x16x32_bf16 emu_mfma_f32_16x16x32_bf16
+#define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4 emu_fp4_pair
+#define __builtin_amdgcn_perm emu_perm
 #define __builtin_amdgcn_update_dpp emu_update_dpp
 #define __builtin_amdgcn_permlane16_swap emu_permlane16_swap
 #define __builtin_amdgcn_permlane32_swap emu_permlane32_swap
 #define __builtin_amdgcn_readfirstlane(x) (x)      /* the kernels use it on wave-uniform values only */
 #define __builtin_amdgcn_ballot_w64 emu_ballot_w64
 #define __builtin_amdgcn_exp2f exp2f
+#define __log2f log2f
 #define __builtin_amdgcn_s_waitcnt emu_s_waitcnt
 #define __builtin_amdgcn_s_barrier emu_s_barrier
 #define __builtin_amdgcn_s_setprio(level) ((void)(level))     // a hint to the instruction arbiter, nothing to emulate
