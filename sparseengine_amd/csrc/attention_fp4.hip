@@ -104,16 +104,6 @@ __device__ __forceinline__ void load_step(Fp4Step<DS>& s, const uint8_t* keys, c
   }
 }
 
-// eight codes (a word) under one factor: an operand's eight bfloat16
-__device__ __forceinline__ bf16x8 operand_of(uint32_t word, uint32_t factor_bits) {
-  uint4 r;
-  r.x = SE_FP4_PAIR(word, factor_bits, 0);
-  r.y = SE_FP4_PAIR(word, factor_bits, 1);
-  r.z = SE_FP4_PAIR(word, factor_bits, 2);
-  r.w = SE_FP4_PAIR(word, factor_bits, 3);
-  return __builtin_bit_cast(bf16x8, r);
-}
-
 // The bytes of eight keys (a pair of dims each), each under its own factor: the operand of the even dim, that of
 // the odd one.
 __device__ __forceinline__ void operands_of(const uint32_t (&codes)[2], const uint32_t (&factors)[2], bf16x8& even, bf16x8& odd) {
@@ -227,7 +217,7 @@ paged_attention_fp4_kernel(const bf16_t* __restrict__ q, int64_t q_stride, const
 #pragma unroll
         for (int ds = 0; ds < DS; ++ds) {
           const uint32_t f = b == 0 ? fp4_factor_bits<0>(s.kf[ds / 4]) : fp4_factor_bits<1>(s.kf[ds / 4]);
-          sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand_of(s.k[b][ds], f),
+          sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fp4_eight(s.k[b][ds], f)),
                                                           __builtin_bit_cast(bf16x8, qf[ds]), sc[b], 0, 0, 0);
         }
       }

@@ -98,3 +98,12 @@ template <int BYTE>
 __device__ __forceinline__ uint32_t fp4_factor_bits(uint32_t word) {   // byte BYTE of `word` as a float's exponent field
   return BYTE < 3 ? word << (23 - 8 * (BYTE < 3 ? BYTE : 0)) : word >> 1;
 }
+// eight codes (a word) under one factor: an operand's eight bfloat16
+__device__ __forceinline__ uint4 fp4_eight(uint32_t word, uint32_t factor_bits) {
+  uint4 r;
+  r.x = SE_FP4_PAIR(word, factor_bits, 0);
+  r.y = SE_FP4_PAIR(word, factor_bits, 1);
+  r.z = SE_FP4_PAIR(word, factor_bits, 2);
+  r.w = SE_FP4_PAIR(word, factor_bits, 3);
+  return r;
+}

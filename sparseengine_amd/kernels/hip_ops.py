@@ -112,9 +112,9 @@ _SIGNATURES = {
         "se_fp4_unpack": [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
     },
     "attention_weights": {
-        # q, q_stride, cache, kind, block_table, bt_stride, item_meta, items, longest, lse, previous, out, heads,
-        # kv_heads, head_dim, page_size, scale, window, dtype, stream
-        "se_attention_weights": [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p,
+        # q, q_stride, cache, kind, block_table, bt_stride, item_meta, items, longest, most_new, lse, previous, out,
+        # heads, kv_heads, head_dim, page_size, scale, window, dtype, stream
+        "se_attention_weights": [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_void_p,
                                  c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
     },
     "evict": {
@@ -553,15 +553,17 @@ class HipKernels:
                  "attention weights: lse must be contiguous float32 [tokens, heads]")
         _require(meta.block_table.dtype == torch.int32 and meta.block_table.dim() == 2 and meta.block_table.stride(1) == 1,
                  "block_table layout")
-        items, longest, item_meta = self._items(meta, tokens, page)
+        if tokens == 0:
+            return
+        items, longest, most_new, item_meta = self._items(meta, tokens, page)
         _same_device(q, cache, lse, out, previous, meta.block_table, item_meta)
         _check(_fn.get("attention_weights", "se_attention_weights")(
             _ptr(q), q.stride(0), _ptr(cache), self._CACHE_KINDS[cache.dtype], _ptr(meta.block_table),
-            meta.block_table.stride(0), _ptr(item_meta), items, longest, _ptr(lse), _ptr(previous), _ptr(out), heads, kv_heads,
+            meta.block_table.stride(0), _ptr(item_meta), items, longest, most_new, _ptr(lse), _ptr(previous), _ptr(out), heads, kv_heads,
             head_dim, page, float(scale), int(window or 0), _code(q.dtype), _stream()), "attention_weights")
 
     def _items(self, meta, tokens: int, page: int):
-        """(number of items, longest context, int32 ``[3, items]`` on the device) of a step, checked."""
+        """(number of items, longest context, most new tokens, int32 ``[3, items]`` on the device) of a step, checked."""
         if getattr(meta, "item_q_len", None) is None:
             raise ValueError("attention weights need the step's items (item_q_len, item_ctx_len)")
         q_len, ctx_len = np.asarray(meta.item_q_len), np.asarray(meta.item_ctx_len)
@@ -576,7 +578,7 @@ class HipKernels:
             item_meta = torch.from_numpy(np.stack([start, q_len, ctx_len]).astype(np.int32)).to(meta.block_table.device)
         _require(item_meta.dtype == torch.int32 and item_meta.is_contiguous() and tuple(item_meta.shape) == (3, q_len.size),
                  "item_meta must be contiguous int32 [3, items]")
-        return q_len.size, longest, item_meta
+        return q_len.size, longest, int(q_len.max()), item_meta
 
     def evict_tokens(self, cache, weights, block_table, lengths, new_table, keep: int, recent: int, kept, longest: int):
         """Of every request's ``lengths[i]`` cached tokens (int32; at most ``longest``) and of every kv head apart, the
