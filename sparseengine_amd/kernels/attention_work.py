@@ -64,6 +64,18 @@ class DeviceAttentionWork:
     tiles_per_block: int
 
 
+# A cache in 4 bits (the same heads; the kernel alone would be bound by reading at one wavefront per SIMD, and a few
+# too many, which run beside the others on some SIMDs, cost as much as twice as many everywhere).  4 requests of up to
+# 131071 keys take 70 us in at most 1024 ranges (6.9 TB/s in the kernel), 78 us in 2048, 85 us in 768; 16 x 16384 keys 44
+# against 49 us; but 64 requests x 8 heads are 512 tiles, whose ranges come in halves: 64 x 8200 keys 150 us unsplit,
+# 88 us in 2048.  A request of 77 keys takes 5.7 us whole and 7.4 in two ranges, 300 keys 9.5 us whole and 8.1 in five.
+# At head size 64 a step has half the bytes and one wavefront per SIMD is not enough (4 x 131071 keys, 32:8 heads: 50 us
+# in 1024 ranges, 43 in 2048).
+FP4_WAVES = 1024            # ranges wanted at head sizes from 128 on, while there are at least four to a tile;
+FP4_MANY_WAVES = 2048       # else
+FP4_MIN_SPLIT_KEYS = 128
+FP4_WHOLE_KEYS = 160        # a step none of whose contexts is longer is not split at all
+
 _native = None      # the compiled builder (csrc/host_work.hip)
 
 
@@ -87,13 +99,14 @@ _BAD_LENGTHS = "attention work: every item needs at least one new token and no m
 
 
 def build_attention_work(q_len, ctx_len, group: int, kv_heads: int, window: int = 0,
-                         target_waves: int = TARGET_WAVES, head_dim: int = 0) -> AttentionWork:
+                         target_waves: int = TARGET_WAVES, head_dim: int = 0,
+                         min_split_keys: int = MIN_SPLIT_KEYS) -> AttentionWork:
     """The work lists of one step, from the compiled builder; ``build_attention_work_numpy`` states
     the rules and gives the same lists (the tests compare the two), about twenty times slower."""
     lib = _native_library()
     q = np.ascontiguousarray(q_len, dtype=np.int64)
     c = np.ascontiguousarray(ctx_len, dtype=np.int64)
-    rules = np.asarray([target_waves, MIN_SPLIT_KEYS, MAX_SPLITS, TILES_PER_BLOCK, TILED_MAX_HEAD_DIM,
+    rules = np.asarray([target_waves, min_split_keys, MAX_SPLITS, TILES_PER_BLOCK, TILED_MAX_HEAD_DIM,
                         TARGET_BLOCKS, MIN_BLOCK_KEYS, PREFIX_PER_PORTION], dtype=np.int64)
     plan = np.empty((q.size, 6), dtype=np.int64)
     counts = np.empty(4, dtype=np.int64)
@@ -113,6 +126,17 @@ def build_attention_work(q_len, ctx_len, group: int, kv_heads: int, window: int 
     return AttentionWork(units, tasks, int(counts[3]), blocks)
 
 
+def build_fp4_attention_work(q_len, ctx_len, group: int, kv_heads: int, window: int = 0, head_dim: int = 0) -> AttentionWork:
+    """The work lists of a step over a cache in 4 bits: ranges that together are no more than fill the chip once (an
+    item's last range is a partial one, so one is taken off the number wanted for each tile)."""
+    q = np.asarray(q_len, dtype=np.int64)
+    tiles = int(((q * group + 15) // 16)[~items_in_blocks(q, group, head_dim)].sum()) * kv_heads
+    wanted = FP4_WAVES if head_dim >= 128 and 4 * tiles <= FP4_WAVES else FP4_MANY_WAVES
+    if q.size and int(np.max(ctx_len)) <= FP4_WHOLE_KEYS:
+        wanted = 0
+    return build_attention_work(q_len, ctx_len, group, kv_heads, window, max(1, wanted - tiles), head_dim, FP4_MIN_SPLIT_KEYS)
+
+
 def items_in_blocks(q_len, group: int, head_dim: int) -> np.ndarray:
     """Which items go to the block kernel: those with at least half a block of tiles."""
     tiles = (np.asarray(q_len, dtype=np.int64) * group + 15) // 16
@@ -122,7 +146,8 @@ def items_in_blocks(q_len, group: int, head_dim: int) -> np.ndarray:
 
 
 def build_attention_work_numpy(q_len, ctx_len, group: int, kv_heads: int, window: int = 0,
-                               target_waves: int = TARGET_WAVES, head_dim: int = 0) -> AttentionWork:
+                               target_waves: int = TARGET_WAVES, head_dim: int = 0,
+                               min_split_keys: int = MIN_SPLIT_KEYS) -> AttentionWork:
     """``head_dim``: 0 keeps every item on the one-wavefront kernel (callers that do not know it).
 
     Items with at least half a block of tiles (prompt portions) go to the block kernel, the others
@@ -155,7 +180,7 @@ def build_attention_work_numpy(q_len, ctx_len, group: int, kv_heads: int, window
     cut = in_blocks & (reach - q_len >= PREFIX_PER_PORTION * q_len)
     whole = int(np.where(cut, 0, nblocks).sum()) * kv_heads
     block_keys = keys_per_unit(np.where(cut, nblocks, 0), TARGET_BLOCKS - whole, MIN_BLOCK_KEYS) if TARGET_BLOCKS > whole else 1 << 30
-    keys = np.where(in_blocks, np.where(cut, block_keys, 1 << 30), keys_per_unit(alone, target_waves, MIN_SPLIT_KEYS))
+    keys = np.where(in_blocks, np.where(cut, block_keys, 1 << 30), keys_per_unit(alone, target_waves, min_split_keys))
     # equal ranges (multiples of 32 keys) over [first_key, ctx) of every item
     first_key = np.maximum(0, ctx_len - reach) // 32 * 32
     span = ctx_len - first_key

@@ -100,10 +100,10 @@ _SIGNATURES = {
                                      c_int, c_void_p],
     },
     "attention_fp4": {
-        # q, q_stride, cache, block_table, bt_stride, units, num_units, out, out_stride, part_o, part_ml, lse,
-        # heads, kv_heads, head_dim, page_size, scale, window, stream
-        "se_paged_attention_fp4": [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64,
-                                   c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p],
+        # q, q_stride, cache, block_table, bt_stride, units, num_units, tasks, num_tasks, out, out_stride, part_o,
+        # part_ml, lse, heads, kv_heads, head_dim, page_size, scale, window, stream
+        "se_paged_attention_fp4": [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
+                                   c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p],
     },
     "cache_fp4": {
         # qkv, row_stride, slots, tokens, heads, kv_heads, head_dim, cache, page_size, dtype, stream
@@ -477,7 +477,8 @@ class HipKernels:
         _require(scale > 0, "attention over a 4-bit cache: scale must be positive")
         direct = q.dtype == torch.bfloat16 and head_dim in self.FP4_HEAD_DIMS
         group = heads // kv_heads
-        work = self._attention_work(q, meta, heads, kv_heads, head_dim, window) if q.dtype == torch.bfloat16 else None
+        work = (self._attention_work(q, meta, heads, kv_heads, head_dim, window, fp4=direct)
+                if q.dtype == torch.bfloat16 else None)
         unpack = None
         if not direct or work.num_block_units:
             unpack = self._fp4_unpack_list(meta, group, head_dim, page, window, only_blocks=direct)
@@ -668,20 +669,22 @@ class HipKernels:
             kv_heads, head_dim, page_size, float(scale), window, _code(q.dtype), _stream()),
             "paged_attention")
 
-    def _attention_work(self, q, meta, heads, kv_heads, head_dim, window):
-        """The step's work lists of the matrix-core kernels, prepared by the batch builder or built here."""
+    def _attention_work(self, q, meta, heads, kv_heads, head_dim, window, fp4=False):
+        """The step's work lists of the matrix-core kernels, prepared by the batch builder or built here.  ``fp4``:
+        those for a cache in 4 bits."""
         group = heads // kv_heads
-        work = None if getattr(meta, "work", None) is None else meta.work.get((group, window))
+        key = (group, window, "fp4") if fp4 else (group, window)
+        work = None if getattr(meta, "work", None) is None else meta.work.get(key)
         if work is None:
-            from .attention_work import DeviceAttentionWork, build_attention_work
-            host = build_attention_work(meta.item_q_len, meta.item_ctx_len, group, kv_heads, window,
-                                        head_dim=head_dim)
+            from .attention_work import DeviceAttentionWork, build_attention_work, build_fp4_attention_work
+            host = (build_fp4_attention_work if fp4 else build_attention_work)(
+                meta.item_q_len, meta.item_ctx_len, group, kv_heads, window, head_dim=head_dim)
             work = DeviceAttentionWork(
                 torch.from_numpy(host.units).to(q.device), host.units.shape[0],
                 torch.from_numpy(host.tasks).to(q.device), host.tasks.shape[0], host.num_slots,
                 torch.from_numpy(host.block_units).to(q.device), host.block_units.shape[0], host.tiles_per_block)
             if getattr(meta, "work", None) is not None:
-                meta.work[(group, window)] = work
+                meta.work[key] = work
         return work
 
     def _run_attention_work(self, q, cache, block_table, work, out, scale, window, lse, fp4=None):
@@ -710,18 +713,20 @@ class HipKernels:
                 _ptr(part_ml), _ptr(lse), heads, kv_heads, head_dim, page_size, float(scale), window,
                 work.tiles_per_block, _stream()), "paged_attention (blocks)",
                 "head_dim a multiple of 32 up to 128, page_size a multiple of 8")
-        units = work.num_units
-        if fp4 is not None and units:
+        if fp4 is not None:
             fp4_cache, fp4_table = fp4
-            _check(_fn.get("attention_fp4", "se_paged_attention_fp4")(
-                _ptr(q), q.stride(0), _ptr(fp4_cache), _ptr(fp4_table), fp4_table.stride(0), _ptr(work.units), units,
-                _ptr(out), out.stride(0), _ptr(part_o), _ptr(part_ml), _ptr(lse), heads, kv_heads, head_dim, page_size,
-                float(scale), window, _stream()), "paged_attention (4-bit cache)", "head_dim 64, 128 or 256")
-            units = 0                         # what is left for the call below: the merges
-        if units or work.num_tasks:           # one wavefront per tile and key range; then all merges
+            if work.num_units or work.num_tasks:
+                _check(_fn.get("attention_fp4", "se_paged_attention_fp4")(
+                    _ptr(q), q.stride(0), _ptr(fp4_cache), _ptr(fp4_table), fp4_table.stride(0),
+                    _ptr(work.units) if work.num_units else None, work.num_units,
+                    _ptr(work.tasks) if work.num_tasks else None, work.num_tasks, _ptr(out), out.stride(0), _ptr(part_o),
+                    _ptr(part_ml), _ptr(lse), heads, kv_heads, head_dim, page_size, float(scale), window, _stream()),
+                    "paged_attention (4-bit cache)", "head_dim 64, 128 or 256, page_size a multiple of 32")
+            return
+        if work.num_units or work.num_tasks:  # one wavefront per tile and key range; then all merges
             _check(_fn.get("attention_mfma", "se_paged_attention_mfma")(
-                _ptr(q), q.stride(0), _ptr(cache), _ptr(block_table), 0 if block_table is None else block_table.stride(0),
-                _ptr(work.units) if units else None, units,
+                _ptr(q), q.stride(0), _ptr(cache), _ptr(block_table), block_table.stride(0),
+                _ptr(work.units) if work.num_units else None, work.num_units,
                 _ptr(work.tasks) if work.num_tasks else None, work.num_tasks, _ptr(out), out.stride(0),
                 _ptr(part_o), _ptr(part_ml), _ptr(lse), heads, kv_heads, head_dim, page_size, float(scale), window,
                 _stream()), "paged_attention (wavefronts)",

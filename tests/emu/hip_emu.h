@@ -566,4 +566,5 @@ inline float emu_max3_bare(float a, float b, float c) { return fmaxf(fmaxf(a, b)
 #define __log2f log2f
 #define __builtin_amdgcn_s_waitcnt emu_s_waitcnt
 #define __builtin_amdgcn_s_barrier emu_s_barrier
+#define __builtin_amdgcn_sched_barrier(mask) ((void)(mask))      // an order for the compiler's scheduler, nothing to emulate
 #define __builtin_amdgcn_s_setprio(level) ((void)(level))     // a hint to the instruction arbiter, nothing to emulate
