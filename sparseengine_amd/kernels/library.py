@@ -114,8 +114,9 @@ def build(names=None, force: bool = False, verbose: bool = True) -> dict[str, Pa
         target = out_dir / f"{name}.{_digest(name)}.so"
         partial = out_dir / f".{name}.{os.getpid()}.tmp.so"
         cmd = [hipcc, *_flags(name), "-o", str(partial), str(CSRC / f"{name}.hip")]
-        proc = subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-        jobs.append((name, proc, partial, target))
+        said = tempfile.TemporaryFile(mode="w+", errors="replace")      # a pipe that nobody empties would stop a talkative compiler
+        proc = subprocess.Popen(cmd, stdout=said, stderr=subprocess.STDOUT)
+        jobs.append((name, proc, partial, target, said))
     if jobs and verbose:
         print(f"[sparseengine_amd] compiling {len(jobs)} kernel librar"
               f"{'y' if len(jobs) == 1 else 'ies'} for {OFFLOAD_ARCH}: "
@@ -125,11 +126,13 @@ def build(names=None, force: bool = False, verbose: bool = True) -> dict[str, Pa
     while pending:
         still = []
         for job in pending:
-            name, proc, partial, target = job
+            name, proc, partial, target, said = job
             if proc.poll() is None:
                 still.append(job)
                 continue
-            output = proc.stdout.read()
+            said.seek(0)
+            output = said.read()
+            said.close()
             if proc.returncode != 0 or not partial.is_file():
                 for other in pending:
                     if other[1].poll() is None:
