@@ -79,31 +79,54 @@ attention_weights_generic_kernel(const T* __restrict__ q, int64_t q_stride, cons
 //                    with four rows of one key and the sum over rows is additions in a lane; the four lanes that
 //                    share a key meet once at the end.
 // With one tile of rows (decoding) a block is four wavefronts side by side along the keys, and the kernel is bound by
-// reading the keys.  With more, the wavefronts of a block take turns at the tiles of the same keys (`row_waves`) and add
-// up their sums through shared memory, in order; the kernel is then bound by the exponentials and the products.
+// the chain of loads in front of its few products: the request's lengths, the page ids, the keys (rows and previous
+// weights are on their way with them).  With more, the wavefronts of a block take turns at the tiles of the same
+// keys (`row_waves`), and several blocks do where there are too few of them to fill the chip evenly (`row_blocks`:
+// their sums go to a workspace and a second kernel adds them up); everything is added in one order, and the kernel is
+// bound by the exponentials and the products.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
-#define WEIGHT_MAX_WAVES 8
+// How a launch goes through the rows.  ONE tile (decoding): no loop, and no rows fetched that are not there.  FEW: rows
+// straight into operands.  MANY: the kernel is bound by vector instructions, of which a tile of 16 rows and 128 keys needs
+// 96 for its exponentials, their arguments and sums, and as much again went into finding its rows; so the 64 lanes
+// find 64 rows (four tiles) at once, and a tile is read row by row (256 contiguous bytes for sixteen lanes) and turned
+// into operands through the wavefront's own part of shared memory (rows 16 bytes apart beyond their length: no two
+// lanes of a read meet in a bank).  2048 rows x 6 heads on 6000 keys: 241 us with rows found and read tile by tile, 195 us
+// so, 0.65 PFLOP/s; the same with 64 keys and three wavefronts per SIMD instead of 128 and two 205 us.
+enum WeightRows { ROWS_ONE = 0, ROWS_FEW = 1, ROWS_MANY = 2 };
 
-template <int DS>
-struct WeightKeys {      // groups of 32 keys a wavefront owns: 64 registers of operands at head size 128
-  static constexpr int KP = DS <= 2 ? 4 : DS <= 4 ? 2 : 1;
+// Groups of 32 keys a wavefront owns: as many as the registers hold where the work that a tile of rows costs whatever the
+// keys is to be shared (MANY at head size 128: 128 registers of operands).
+template <int DS, int MODE>
+struct WeightShape {
+  static constexpr int KP = MODE == ROWS_MANY ? (DS == 1 ? 8 : DS <= 4 ? 4 : DS <= 6 ? 2 : 1)
+                            : MODE == ROWS_ONE ? (DS == 1 ? 8 : DS == 2 ? 6 : DS <= 4 ? 4 : 2)
+                                               : (DS <= 2 ? 4 : DS <= 4 ? 2 : 1);
+  static constexpr int WAVES = 4;      // of a block
+  static constexpr int PER_SIMD = MODE == ROWS_MANY ? 2 : 1;
 };
 
-template <int DS, int KIND>
-__global__ void __launch_bounds__(64 * WEIGHT_MAX_WAVES)
+template <int DS, int KIND, int MODE>
+__global__ void __launch_bounds__((64 * WeightShape<DS, MODE>::WAVES), (WeightShape<DS, MODE>::PER_SIMD))
 attention_weights_mfma_kernel(const bf16_t* __restrict__ q, int64_t q_stride, const void* __restrict__ cache,
                               const int32_t* __restrict__ block_table, int bt_stride,
                               const int32_t* __restrict__ item_meta, int items, int longest,
                               const float* __restrict__ lse, const float* previous, float* out, int heads, int kv_heads,
-                              int page_size, float scale_log2e, int window, int row_waves) {
+                              int page_size, float scale_log2e, int window, int row_waves, int row_blocks,
+                              float* __restrict__ partial) {
   constexpr int D = 32 * DS;
-  constexpr int KP = WeightKeys<DS>::KP;
+  constexpr int KP = WeightShape<DS, MODE>::KP, waves = WeightShape<DS, MODE>::WAVES;
+  constexpr int ROW_BYTES = 64 * DS + 16;      // of a row in shared memory
   // which eight dims of a lane's operand are those of product step ds: in 4 bits, where a lane's part of a key can be
   // one piece under one factor, neighbouring ones
   constexpr bool WIDE = KIND == SE_CACHE_FP4 && (DS == 2 || DS == 4 || DS == 8);
-  __shared__ float sums[WEIGHT_MAX_WAVES][KP * 2][16];
+  __shared__ float sums[waves][KP * 2][16];
+  constexpr int INFO = MODE == ROWS_MANY ? waves : 1;
+  __shared__ __align__(16) int64_t row_places[INFO][2][64];
+  __shared__ __align__(16) float row_lse2[INFO][2][64];
+  __shared__ __align__(16) int row_pos[INFO][2][64];
+  __shared__ __align__(16) unsigned char staged[MODE == ROWS_MANY ? waves * 16 * ROW_BYTES : 16];
   const int lane = threadIdx.x & (SE_WAVE - 1);
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / SE_WAVE));
   const int n = lane & 15, g = lane >> 4;
@@ -111,9 +134,9 @@ attention_weights_mfma_kernel(const bf16_t* __restrict__ q, int64_t q_stride, co
   const int q_start = item_meta[item], q_len = item_meta[items + item], ctx_len = min(item_meta[2 * items + item], longest);
   const int pos0 = ctx_len - q_len, last_key = ctx_len - 1;
   const int low_key = window > 0 && pos0 - window + 1 > 0 ? pos0 - window + 1 : 0;   // no row sees a key before it
-  const int waves = blockDim.x / SE_WAVE;
-  const int part = wave % row_waves;                                                 // of the rows
-  const int k_lo = (blockIdx.x * (waves / row_waves) + wave / row_waves) * (32 * KP), k_hi = k_lo + 32 * KP - 1;
+  const int row_block = blockIdx.x % row_blocks, key_block = blockIdx.x / row_blocks;
+  const int part = wave % row_waves;                                                 // of the block's share of the rows
+  const int k_lo = (key_block * (waves / row_waves) + wave / row_waves) * (32 * KP), k_hi = k_lo + 32 * KP - 1;
   const bool wanted = k_lo < ctx_len && k_hi >= low_key;      // the same in all wavefronts that share keys
   const int32_t* table = block_table + static_cast<int64_t>(item) * bt_stride;
 
@@ -121,11 +144,63 @@ attention_weights_mfma_kernel(const bf16_t* __restrict__ q, int64_t q_stride, co
   // a lane's keys: two neighbours in 4 bits (one piece of memory), else sixteen lanes side by side
   auto key_of = [&](int kp, int b) { return k_lo + 32 * kp + (KIND == SE_CACHE_FP4 ? 2 * n + b : 16 * b + n); };
 
-  float acc[KP][2];
+  // where a lane's key has its weight (some held key's for one that is not held)
+  auto place_of = [&](int kp, int b) {
+    if constexpr (KIND == SE_CACHE_FP4) {      // 32 keys lie in one page: scalar work
+      const int first = max(min(k_lo + 32 * kp, last_key & ~31), low_key & ~31);
+      return (static_cast<int64_t>(table[first / page_size]) * kv_heads + kvh) * page_size + first % page_size + 2 * n + b;
+    } else {
+      const int key = max(min(key_of(kp, b), last_key), low_key);
+      return (static_cast<int64_t>(table[key / page_size]) * kv_heads + kvh) * page_size + key % page_size;
+    }
+  };
+
+  float acc[KP][2], before[KP][2];
+  int64_t place[KP][2];
 #pragma unroll
-  for (int kp = 0; kp < KP; ++kp) acc[kp][0] = acc[kp][1] = 0.f;
+  for (int kp = 0; kp < KP; ++kp) acc[kp][0] = acc[kp][1] = before[kp][0] = before[kp][1] = 0.f;
 
   if (wanted) {
+    // the tiles with a row that sees one of the keys
+    const int rows_total = q_len * group;
+    int tile = k_lo > pos0 ? static_cast<int>(static_cast<int64_t>(k_lo - pos0) * group / 16) : 0;
+    int until = (rows_total + 15) / 16;
+    if (window > 0) {
+      const int64_t last_q = static_cast<int64_t>(min(k_hi, last_key)) + window - 1 - pos0;
+      if (last_q + 1 < q_len) until = static_cast<int>(((last_q + 1) * group + 15) / 16);
+    }
+    struct Rows {
+      uint4 q[DS];     // the lane's operands (MANY: not used)
+      int64_t at;      // where its row begins (MANY only)
+      float lse;       // of that row
+      int pos, rho;    // rho >= rows_total: there is no such row
+    };
+    // a lane's row of the next tile to be fetched: row `rho` of the request is head `row_head` of token `row_token`
+    if constexpr (MODE != ROWS_MANY) tile += row_block * row_waves + part;
+    const int tile_step = row_waves * row_blocks;
+    int rho = tile * 16 + n;
+    int row_token = rho / group, row_head = rho - row_token * group;
+    const int step = tile_step * 16, step_tokens = step / group, step_heads = step - step_tokens * group;
+    auto fetch = [&](Rows& r) {      // the wavefront's tiles, one after the other
+      const bool valid = rho < rows_total;
+      const int q_idx = valid ? row_token : q_len - 1, head = kvh * group + (valid ? row_head : group - 1);
+      const int64_t row_at = static_cast<int64_t>(q_start + q_idx) * q_stride + static_cast<int64_t>(head) * D;
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds) r.q[ds] = *reinterpret_cast<const uint4*>(q + row_at + dims_of(ds));
+      r.lse = lse[static_cast<int64_t>(q_start + q_idx) * heads + head];   // not looked at here: that would be a wait
+      r.pos = pos0 + q_idx;
+      r.rho = rho;
+      rho += step;
+      row_token += step_tokens;
+      row_head += step_heads;
+      if (row_head >= group) {
+        row_head -= group;
+        ++row_token;
+      }
+    };
+    Rows a, b;      // the next tile's rows are on their way while one is worked on; beyond the last tile the last row once more
+    if constexpr (MODE != ROWS_MANY) fetch(a);
+    if constexpr (MODE == ROWS_FEW) fetch(b);
     uint4 kf[KP][2][DS];
     if constexpr (KIND == SE_CACHE_FP4) {
       const int64_t head_bytes = fp4_head_bytes(page_size, D), factors = fp4_factors_at(page_size, D);
@@ -183,30 +258,18 @@ attention_weights_mfma_kernel(const bf16_t* __restrict__ q, int64_t q_stride, co
         }
     }
 
-    // the tiles with a row that sees one of the keys
-    const int rows_total = q_len * group;
-    int tile = k_lo > pos0 ? static_cast<int>(static_cast<int64_t>(k_lo - pos0) * group / 16) : 0;
-    int until = (rows_total + 15) / 16;
-    if (window > 0) {
-      const int64_t last_q = static_cast<int64_t>(min(k_hi, last_key)) + window - 1 - pos0;
-      if (last_q + 1 < q_len) until = static_cast<int>(((last_q + 1) * group + 15) / 16);
-    }
-    struct Rows {
-      uint4 q[DS];
-      float lse2;      // of the lane's row n, in powers of two; +inf: there is no such row
-      int pos;
-    };
-    auto fetch = [&](Rows& r, int t) {
-      const int rho = t * 16 + n, rho_c = min(rho, rows_total - 1);
-      const int q_idx = rho_c / group, head = kvh * group + rho_c - q_idx * group;
-      const bf16_t* row = q + static_cast<int64_t>(q_start + q_idx) * q_stride + static_cast<int64_t>(head) * D;
+    if (MODE == ROWS_ONE && g == 0) {      // on their way with the keys
 #pragma unroll
-      for (int ds = 0; ds < DS; ++ds) r.q[ds] = *reinterpret_cast<const uint4*>(row + dims_of(ds));
-      const float l = lse[static_cast<int64_t>(q_start + q_idx) * heads + head];
-      r.lse2 = rho < rows_total ? l * 1.4426950408889634f : INFINITY;
-      r.pos = pos0 + q_idx;
-    };
-    auto weigh = [&](const Rows& r, int t) {
+      for (int kp = 0; kp < KP; ++kp)
+#pragma unroll
+        for (int b2 = 0; b2 < 2; ++b2) {
+          place[kp][b2] = place_of(kp, b2);
+          const int key = key_of(kp, b2);
+          if (previous != nullptr && key < pos0 && key >= low_key) before[kp][b2] = previous[place[kp][b2]];
+        }
+    }
+    // rows: a lane's operand of row n; l, pos: lse (in powers of two) and position of rows 4 g + i
+    auto weigh = [&](const uint4 (&rows)[DS], const float (&l)[4], const int (&pos)[4], bool some_hidden) {
       floatx4 s[KP][2];
 #pragma unroll
       for (int kp = 0; kp < KP; ++kp)
@@ -215,24 +278,20 @@ attention_weights_mfma_kernel(const bf16_t* __restrict__ q, int64_t q_stride, co
           s[kp][b] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int ds = 0; ds < DS; ++ds)
-            s[kp][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, r.q[ds]),
+            s[kp][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, rows[ds]),
                                                                __builtin_bit_cast(bf16x8, kf[kp][b][ds]), s[kp][b], 0, 0, 0);
         }
       // lane (g, n): s[kp][b][i] is the score of row 4 g + i for key key_of(kp, b)
-      float l[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) l[i] = __shfl(r.lse2, 4 * g + i, SE_WAVE);
-      const int pos_min = pos0 + t * 16 / group, pos_max = pos0 + min(t * 16 + 15, rows_total - 1) / group;
-      if (k_hi > pos_min || (window > 0 && k_lo <= pos_max - window)) {      // the same in all lanes
+      if (__builtin_expect(some_hidden, 0)) {      // the same in all lanes
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int pos = __shfl(r.pos, 4 * g + i, SE_WAVE);
+          const int hidden = window > 0 ? pos[i] - window : -1;      // the last key too old
 #pragma unroll
           for (int kp = 0; kp < KP; ++kp)
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
               const int key = key_of(kp, b);
-              if (key > pos || (window > 0 && key <= pos - window)) s[kp][b][i] = -INFINITY;
+              s[kp][b][i] = ((key > pos[i]) | (key <= hidden)) ? -INFINITY : s[kp][b][i];
             }
         }
       }
@@ -246,18 +305,96 @@ attention_weights_mfma_kernel(const bf16_t* __restrict__ q, int64_t q_stride, co
           acc[kp][b] += sum;
         }
     };
-    tile += part;
-    if (tile < until) {
-      Rows a, b;
-      fetch(a, tile);
-      for (; tile < until; tile += 2 * row_waves) {      // the next tile's rows are on their way meanwhile
-        const bool second = tile + row_waves < until;
-        if (second) fetch(b, tile + row_waves);
-        weigh(a, tile);
-        if (!second) break;
-        if (tile + 2 * row_waves < until) fetch(a, tile + 2 * row_waves);
-        weigh(b, tile + row_waves);
+    // (No way out from the middle of a round: the wait at its head would be one for the loads just issued.)
+    auto weigh_tile = [&](const Rows& r) {
+      const float lse2 = r.rho < rows_total ? r.lse * 1.4426950408889634f : INFINITY;     // in powers of two
+      float l[4];
+      int pos[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l[i] = __shfl(lse2, 4 * g + i, SE_WAVE), pos[i] = __shfl(r.pos, 4 * g + i, SE_WAVE);
+      const int pos_min = __builtin_amdgcn_readlane(r.pos, 0), pos_max = __builtin_amdgcn_readlane(r.pos, 15);
+      weigh(r.q, l, pos, k_hi > pos_min || (window > 0 && k_lo <= pos_max - window));
+    };
+    if constexpr (MODE == ROWS_ONE) {
+      if (tile < until) weigh_tile(a);
+    } else if constexpr (MODE == ROWS_FEW) {
+      for (; tile < until; tile += 2 * tile_step) {
+        weigh_tile(a);
+        fetch(a);
+        if (tile + tile_step < until) weigh_tile(b);
+        fetch(b);
       }
+    } else {
+      // Four tiles at a time: lane l works out where row l of the 64 lies, its lse and its position, for the four tiles
+      // after those at hand, and leaves them in the wavefront's own shared memory (a wavefront's own accesses to it stay
+      // in their order).  The tile after the one at hand is on its way: its vectors lane, 64 + lane, ... in the order of
+      // its rows.  (A macro and plain vectors of this scope: an array of them that a lambda fills through a reference, or of
+      // the runtime's vector type, ends up in scratch memory.)
+      const int groups_until = (until + 3) / 4, group_step = tile_step;
+      int row_group = tile / 4 + row_block * row_waves + part;      // of 64 rows
+      unsigned char* mine = staged + wave * 16 * ROW_BYTES;
+      int64_t(*places)[64] = row_places[wave];
+      float(*lse2)[64] = row_lse2[wave];
+      int(*positions)[64] = row_pos[wave];
+      Rows info;
+      info.rho = 0;
+      rho = row_group * 64 + lane;
+      row_token = rho / group, row_head = rho - row_token * group;
+      const int info_step = group_step * 64, info_tokens = info_step / group, info_heads = info_step - info_tokens * group;
+      auto ask = [&]() {
+        const bool valid = rho < rows_total;
+        const int q_idx = valid ? row_token : q_len - 1, head = kvh * group + (valid ? row_head : group - 1);
+        info.at = static_cast<int64_t>(q_start + q_idx) * q_stride + static_cast<int64_t>(head) * D;
+        info.lse = lse[static_cast<int64_t>(q_start + q_idx) * heads + head];
+        info.pos = pos0 + q_idx;
+        info.rho = rho;
+        rho += info_step;
+        row_token += info_tokens;
+        row_head += info_heads;
+        if (row_head >= group) row_head -= group, ++row_token;
+      };
+      auto keep_info = [&](int buffer) {
+        places[buffer][lane] = info.at;
+        lse2[buffer][lane] = info.rho < rows_total ? info.lse * 1.4426950408889634f : INFINITY;    // +inf: there is no such row
+        positions[buffer][lane] = info.pos;
+      };
+      se_u32x4 next[DS];
+#define WEIGHT_READ_ROWS(BUFFER, TILE)                                                                                    \
+  _Pragma("unroll") for (int i = 0; i < DS; ++i)                                                                          \
+      next[i] = *reinterpret_cast<const se_u32x4*>(q + places[BUFFER][16 * (TILE) + (64 * i + lane) / (4 * DS)] +         \
+                                                   (64 * i + lane) % (4 * DS) * 8);
+      int buffer = 0;
+      if (row_group < groups_until) {
+        ask();
+        keep_info(0);
+        __builtin_amdgcn_wave_barrier();
+        WEIGHT_READ_ROWS(0, 0)
+      }
+      for (; row_group < groups_until; row_group += group_step, buffer ^= 1) {
+        const int pos_min = __builtin_amdgcn_readfirstlane(positions[buffer][0]);
+        const int pos_max = __builtin_amdgcn_readfirstlane(positions[buffer][63]);
+        const bool some_hidden = k_hi > pos_min || (window > 0 && k_lo <= pos_max - window);      // from some of the 64 rows
+        ask();      // beyond the last rows: the last one
+#pragma unroll 1      // four copies of the body would hoist each other's work into more registers than there are
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+          for (int i = 0; i < DS; ++i)
+            *reinterpret_cast<se_u32x4*>(mine + (64 * i + lane) / (4 * DS) * ROW_BYTES + (64 * i + lane) % (4 * DS) * 16) = next[i];
+          if (t == 2) keep_info(buffer ^ 1);
+          __builtin_amdgcn_wave_barrier();
+          WEIGHT_READ_ROWS((t < 3 ? buffer : buffer ^ 1), (t + 1 & 3))
+          uint4 rows[DS];
+#pragma unroll
+          for (int ds = 0; ds < DS; ++ds) rows[ds] = *reinterpret_cast<const uint4*>(mine + n * ROW_BYTES + dims_of(ds) * 2);
+          const float4 l4 = *reinterpret_cast<const float4*>(&lse2[buffer][16 * t + 4 * g]);
+          const int4 p4 = *reinterpret_cast<const int4*>(&positions[buffer][16 * t + 4 * g]);
+          __builtin_amdgcn_wave_barrier();
+          const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+          const int p[4] = {p4.x, p4.y, p4.z, p4.w};
+          weigh(rows, l, p, some_hidden);
+        }
+      }
+#undef WEIGHT_READ_ROWS
     }
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp)
@@ -287,36 +424,93 @@ attention_weights_mfma_kernel(const bf16_t* __restrict__ q, int64_t q_stride, co
     for (int b = 0; b < 2; ++b) {
       const int key = key_of(kp, b);
       if (key > last_key || key < low_key) continue;
-      const int64_t at = (static_cast<int64_t>(table[key / page_size]) * kv_heads + kvh) * page_size + key % page_size;
-      out[at] = (previous != nullptr && key < pos0 ? previous[at] : 0.f) + acc[kp][b];
+      if (row_blocks > 1) {
+        partial[((static_cast<int64_t>(row_block) * items + item) * kv_heads + kvh) * longest + key] = acc[kp][b];
+        continue;
+      }
+      if constexpr (MODE == ROWS_ONE) {
+        out[place[kp][b]] = before[kp][b] + acc[kp][b];
+      } else {
+        const int64_t at = place_of(kp, b);
+        out[at] = (previous != nullptr && key < pos0 ? previous[at] : 0.f) + acc[kp][b];
+      }
     }
+}
+
+// Adds up the sums of `row_blocks` blocks of every key.
+__global__ void __launch_bounds__(256)
+join_weights_kernel(const float* __restrict__ partial, int row_blocks, const int32_t* __restrict__ block_table, int bt_stride,
+                    const int32_t* __restrict__ item_meta, int items, int longest, const float* previous, float* out,
+                    int kv_heads, int page_size, int window) {
+  const int item = blockIdx.z, kvh = blockIdx.y, key = blockIdx.x * blockDim.x + threadIdx.x;
+  const int q_len = item_meta[items + item], ctx_len = min(item_meta[2 * items + item], longest), pos0 = ctx_len - q_len;
+  const int low_key = window > 0 && pos0 - window + 1 > 0 ? pos0 - window + 1 : 0;
+  if (key >= ctx_len || key < low_key) return;
+  float sum = 0.f;
+  for (int s = 0; s < row_blocks; ++s) sum += partial[((static_cast<int64_t>(s) * items + item) * kv_heads + kvh) * longest + key];
+  const int page = block_table[static_cast<int64_t>(item) * bt_stride + key / page_size];
+  const int64_t at = (static_cast<int64_t>(page) * kv_heads + kvh) * page_size + key % page_size;
+  out[at] = (previous != nullptr && key < pos0 ? previous[at] : 0.f) + sum;
+}
+
+// Blocks that share the rows of the same keys: enough for six rounds of one block of eight wavefronts per CU, as long
+// as a wavefront has at least four tiles (2048 rows x 6 heads on 6000 keys, 8 kv heads: 376 blocks alone run in one
+// round and a half, 241 us).
+#define WEIGHT_BLOCKS 1536
+static int many_rows_keys(int head_dim) {      // of a wavefront, as WeightShape has it
+  const int ds = head_dim / 32;
+  return 32 * (ds == 1 ? 8 : ds <= 4 ? 4 : ds <= 6 ? 2 : 1);
+}
+static bool weights_on_matrix_cores(int head_dim, int64_t most_rows, int dtype) {
+  return dtype == SE_BF16 && head_dim % 32 == 0 && head_dim <= 256 && most_rows < 0x40000000;
+}
+// How many sums of every key a call leaves in its workspace: float [that, items, kv_heads, longest] (1: none is used).
+extern "C" int se_attention_weights_splits(int items, int longest, int most_new, int heads, int kv_heads, int head_dim, int dtype) {
+  if (items <= 0 || longest <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0) return 1;
+  const int64_t most_rows = static_cast<int64_t>(most_new) * (heads / kv_heads);
+  const int64_t tiles = (most_rows + 15) / 16;
+  if (!weights_on_matrix_cores(head_dim, most_rows, dtype) || tiles <= 32) return 1;
+  const int64_t keys = many_rows_keys(head_dim);
+  const int64_t blocks = (longest + keys - 1) / keys * kv_heads * items;
+  int64_t splits = (WEIGHT_BLOCKS + blocks - 1) / blocks;
+  if (splits > tiles / 32) splits = tiles / 32;
+  return splits < 1 ? 1 : splits > 16 ? 16 : static_cast<int>(splits);
 }
 
 template <int DS, int KIND>
 static void launch_weights_mfma(const void* q, int64_t q_stride, const void* cache, const int32_t* block_table, int bt_stride,
                                 const int32_t* item_meta, int items, int longest, int most_rows, const float* lse,
                                 const float* previous, float* out, int heads, int kv_heads, int page_size, float scale,
-                                int window, hipStream_t stream) {
-  constexpr int keys = 32 * WeightKeys<DS>::KP;
+                                int window, int splits, float* partial, hipStream_t stream) {
   // With a single tile there is nothing to share out among the wavefronts of the same keys.
   const int tiles = (most_rows + 15) / 16;
-  const int row_waves = tiles <= 1 ? 1 : tiles <= 8 ? 2 : tiles <= 32 ? 4 : 8;
-  const int waves = row_waves < 4 ? 4 : row_waves;
-  const int per_block = keys * (waves / row_waves);
-  const dim3 grid((longest + per_block - 1) / per_block, kv_heads, items);
-  attention_weights_mfma_kernel<DS, KIND><<<grid, waves * SE_WAVE, 0, stream>>>(
-      static_cast<const bf16_t*>(q), q_stride, cache, block_table, bt_stride, item_meta, items, longest, lse, previous, out,
-      heads, kv_heads, page_size, scale * 1.4426950408889634f, window, row_waves);
+#define SE_WEIGHTS_LAUNCH(MODE, ROW_WAVES, ROW_BLOCKS)                                                                     \
+  {                                                                                                                        \
+    constexpr int waves = WeightShape<DS, MODE>::WAVES;                                                                    \
+    const int per_block = 32 * WeightShape<DS, MODE>::KP * (waves / (ROW_WAVES));                                          \
+    const dim3 grid((longest + per_block - 1) / per_block * (ROW_BLOCKS), kv_heads, items);                                \
+    attention_weights_mfma_kernel<DS, KIND, MODE><<<grid, waves * SE_WAVE, 0, stream>>>(                                   \
+        static_cast<const bf16_t*>(q), q_stride, cache, block_table, bt_stride, item_meta, items, longest, lse, previous, out, \
+        heads, kv_heads, page_size, scale * 1.4426950408889634f, window, ROW_WAVES, ROW_BLOCKS, partial);                  \
+  }
+  if (tiles <= 1) SE_WEIGHTS_LAUNCH(ROWS_ONE, 1, 1)
+  else if (tiles <= 8) SE_WEIGHTS_LAUNCH(ROWS_FEW, 2, 1)
+  else if (tiles <= 32) SE_WEIGHTS_LAUNCH(ROWS_FEW, 4, 1)
+  else SE_WEIGHTS_LAUNCH(ROWS_MANY, waves, splits)
+#undef SE_WEIGHTS_LAUNCH
+  if (splits > 1)
+    join_weights_kernel<<<dim3((longest + 255) / 256, kv_heads, items), 256, 0, stream>>>(
+        partial, splits, block_table, bt_stride, item_meta, items, longest, previous, out, kv_heads, page_size, window);
 }
 
 // q [.., heads, head_dim] with token stride q_stride; cache of `kind` (SeCacheKind); item_meta int32 [3, items]:
 // first token, new tokens and tokens with them of every request; longest: the largest of the latter; most_new: the
-// largest of the new ones.
+// largest of the new ones; workspace: what se_attention_weights_splits says.
 extern "C" int se_attention_weights(const void* q, int64_t q_stride, const void* cache, int kind,
                                     const int32_t* block_table, int bt_stride, const int32_t* item_meta, int items,
                                     int longest, int most_new, const float* lse, const float* previous, float* out, int heads,
                                     int kv_heads, int head_dim, int page_size, float scale, int window, int dtype,
-                                    hipStream_t stream) {
+                                    float* workspace, hipStream_t stream) {
   if (items <= 0 || longest <= 0) return SE_OK;
   if (head_dim <= 0 || head_dim % 8 || head_dim > 512) return SE_ERR_SHAPE;
   if (kv_heads <= 0 || heads % kv_heads || page_size <= 0 || page_size % 8) return SE_ERR_SHAPE;
@@ -324,10 +518,12 @@ extern "C" int se_attention_weights(const void* q, int64_t q_stride, const void*
   if (kind != SE_CACHE_FP4 && kind != (dtype == SE_F32 ? SE_CACHE_F32 : SE_CACHE_BF16)) return SE_ERR_SHAPE;
   if (kv_heads > 65535 || items > 65535) return SE_ERR_SHAPE;
   const int64_t most_rows = static_cast<int64_t>(most_new) * (heads / kv_heads);
-  if (dtype == SE_BF16 && head_dim % 32 == 0 && head_dim <= 256 && most_rows < 0x40000000) {
+  if (weights_on_matrix_cores(head_dim, most_rows, dtype)) {
+    const int splits = se_attention_weights_splits(items, longest, most_new, heads, kv_heads, head_dim, dtype);
+    if (splits > 1 && workspace == nullptr) return SE_ERR_SHAPE;
 #define SE_WEIGHTS_MFMA(DS, KIND)                                                                                   \
   launch_weights_mfma<DS, KIND>(q, q_stride, cache, block_table, bt_stride, item_meta, items, longest,              \
-                                static_cast<int>(most_rows), lse, previous, out, heads, kv_heads, page_size, scale, window, stream)
+                                static_cast<int>(most_rows), lse, previous, out, heads, kv_heads, page_size, scale, window, splits, workspace, stream)
 #define SE_WEIGHTS_CASE(DS)                                     \
   case DS:                                                      \
     if (kind == SE_CACHE_FP4) SE_WEIGHTS_MFMA(DS, SE_CACHE_FP4); \

@@ -1,10 +1,13 @@
 // Letting tokens go: of every request and kv head the last `recent` tokens and the heaviest of the others, `keep` in
 // all, are moved to other pages in their order, with their weights.
 //
-//   choose   one block per (request, kv head).  The weights are ordered as unsigned words (negative
-//            below positive, not-a-number above all); the smallest that is kept is found eight bits at a
-//            time by counting how many candidates share the bits found so far, and among equal ones the first are
-//            kept.  Integer counts only: the result does not depend on the order in which the threads count.
+//   choose   one block per (request, kv head).  The weights are ordered as unsigned words (negative below positive,
+//            not-a-number above all), read once and kept in registers (up to 32768 tokens; the rest is read again in
+//            every pass).  The smallest word that is kept is found eight bits a pass from counts of the candidates
+//            that share the bits found so far (integer additions in shared memory, sixteen copies of every count so
+//            that the crowd of words with one exponent does not queue up at one address); the search ends early when
+//            the words at or above the one found are just those wanted, and among words equal to the smallest the
+//            first are kept.  Whole numbers only: the result does not depend on the order in which threads count.
 //   move     the chosen tokens' keys, values, factors and weights, gathered into the new pages.
 //
 // `weights` lies in pages beside the cache: [pages, kv_heads, page_size] float.  The new pages must not be among the
@@ -20,14 +23,40 @@ __device__ __forceinline__ uint32_t order_word(float w) {     // larger weights,
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
+#define CHOOSE_WAVES (CHOOSE_THREADS / SE_WAVE)
+#define CHOOSE_COPIES 16
+
+// Exclusive prefix sums of `counts` [rounds][CHOOSE_WAVES] in place, and their sum; entries <= CHOOSE_THREADS.
+__device__ __forceinline__ int scan_counts(int* counts, int entries, int* wave_sums) {
+  const int tid = threadIdx.x, lane = tid & (SE_WAVE - 1), wave = tid / SE_WAVE;
+  const int own = tid < entries ? counts[tid] : 0;
+  int upto = own;
+#pragma unroll
+  for (int off = 1; off < SE_WAVE; off <<= 1) {
+    const int other = __shfl_up(upto, off, SE_WAVE);
+    if (lane >= off) upto += other;
+  }
+  if (lane == SE_WAVE - 1) wave_sums[wave] = upto;
+  __syncthreads();
+  int before = 0, total = 0;
+  for (int w = 0; w < CHOOSE_WAVES; ++w) {
+    if (w < wave) before += wave_sums[w];
+    total += wave_sums[w];
+  }
+  if (tid < entries) counts[tid] = before + upto - own;
+  __syncthreads();
+  return total;
+}
+
+// R: words a thread keeps in registers; tokens beyond R * CHOOSE_THREADS are read again whenever they are looked at.
+template <int R>
 __global__ void __launch_bounds__(CHOOSE_THREADS)
 choose_tokens_kernel(const float* __restrict__ weights, const int32_t* __restrict__ block_table, int bt_stride,
                      const int32_t* __restrict__ lengths, int longest, int kv_heads, int page_size, int keep, int recent,
                      int32_t* __restrict__ kept) {
-  __shared__ int bins[256];
-  __shared__ int wave_counts[2][CHOOSE_THREADS / SE_WAVE];
-  __shared__ uint32_t found_prefix;
-  __shared__ int found_above;
+  __shared__ int round_counts[R * CHOOSE_WAVES];      // per (round of CHOOSE_THREADS tokens, wavefront)
+  __shared__ int wave_counts[2][CHOOSE_WAVES];
+  __shared__ int bins[256 * CHOOSE_COPIES], own_sum[256], upto_sum[256], found[3];
   const int item = blockIdx.y, kvh = blockIdx.x, tid = threadIdx.x;
   const int lane = tid & (SE_WAVE - 1), wave = tid / SE_WAVE;
   const int length = min(lengths[item], longest);      // the block table's rows hold `longest` tokens
@@ -40,67 +69,129 @@ choose_tokens_kernel(const float* __restrict__ weights, const int32_t* __restric
   const int late = recent < keep ? recent : keep;
   const int candidates = length - late;      // tokens before the recent ones
   const int want = keep - late;              // of which so many stay (fewer than all: length > keep)
-  auto word_at = [&](int i) {
-    return order_word(weights[(static_cast<int64_t>(table[i / page_size]) * kv_heads + kvh) * page_size + i % page_size]);
+  // The words of tokens base + tid, base + tid + CHOOSE_THREADS, ...: 0, which is no weight's word, for what is no
+  // candidate.  The page of the next token is found by adding, not by dividing.
+  const int step_pages = CHOOSE_THREADS / page_size, step_off = CHOOSE_THREADS - step_pages * page_size;
+  auto read_words = [&](int base, uint32_t (&word)[R]) {
+    int page = (base + tid) / page_size, off = (base + tid) - page * page_size;
+    int id[R], at[R];       // all page ids on their way at once, then all weights (the first token's for no candidate)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool candidate = base + r * CHOOSE_THREADS + tid < candidates;
+      id[r] = table[candidate ? page : 0];
+      at[r] = candidate ? off : 0;
+      page += step_pages;
+      off += step_off;
+      if (off >= page_size) {
+        off -= page_size;
+        ++page;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float w = weights[(static_cast<int64_t>(id[r]) * kv_heads + kvh) * page_size + at[r]];
+      word[r] = base + r * CHOOSE_THREADS + tid < candidates ? order_word(w) : 0u;
+    }
   };
-  // the want-th largest word: the bits found so far, and how many candidates lie above everything that shares them
-  uint32_t prefix = 0;
-  int above = 0;
-  if (want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += CHOOSE_THREADS) bins[i] = 0;
-      __syncthreads();
-      const uint32_t high = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-      for (int i = tid; i < candidates; i += CHOOSE_THREADS) {
-        const uint32_t w = word_at(i);
-        if ((w & high) == prefix) atomicAdd(&bins[w >> shift & 255u], 1);
+  uint32_t word[R];
+  read_words(0, word);
+
+  // the want-th largest word, and how many candidates lie at or above it
+  uint32_t least = 0;
+  int above = 0, at_or_above = 0;      // above: of the candidates that do not share the bits found so far
+  for (int shift = 24; want > 0 && shift >= 0 && at_or_above != want; shift -= 8) {
+    const uint32_t high = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
+    for (int i = tid; i < 256 * CHOOSE_COPIES; i += CHOOSE_THREADS) bins[i] = 0;
+    __syncthreads();
+    auto count = [&](uint32_t w) {
+      if (w != 0 && (w & high) == least) atomicAdd(&bins[(w >> shift & 255u) * CHOOSE_COPIES + lane % CHOOSE_COPIES], 1);
+    };
+#pragma unroll
+    for (int r = 0; r < R; ++r) count(word[r]);
+    int page = (R * CHOOSE_THREADS + tid) / page_size, off = (R * CHOOSE_THREADS + tid) - page * page_size;
+    for (int i = R * CHOOSE_THREADS + tid; i < candidates; i += CHOOSE_THREADS) {
+      count(order_word(weights[(static_cast<int64_t>(table[page]) * kv_heads + kvh) * page_size + off]));
+      page += step_pages;
+      off += step_off;
+      if (off >= page_size) {
+        off -= page_size;
+        ++page;
       }
-      __syncthreads();
-      if (tid == 0) {
-        int sum = above, b = 255;
-        while (b > 0 && sum + bins[b] < want) sum += bins[b--];
-        found_prefix = prefix | static_cast<uint32_t>(b) << shift;
-        found_above = sum;
-      }
-      __syncthreads();
-      prefix = found_prefix;
-      above = found_above;
     }
+    __syncthreads();
+    if (tid < 256) {      // thread t: bin 255 - t, so that sums run from the largest words down
+      int own = 0;
+#pragma unroll
+      for (int c = 0; c < CHOOSE_COPIES; ++c) own += bins[(255 - tid) * CHOOSE_COPIES + c];
+      int upto = own;
+#pragma unroll
+      for (int off = 1; off < SE_WAVE; off <<= 1) {
+        const int other = __shfl_up(upto, off, SE_WAVE);
+        if (lane >= off) upto += other;
+      }
+      own_sum[tid] = own;
+      upto_sum[tid] = upto;
+    }
+    __syncthreads();
+    if (tid < 256) {
+      int upto = above + upto_sum[tid];
+      for (int w = 0; w < tid / SE_WAVE; ++w) upto += upto_sum[w * SE_WAVE + SE_WAVE - 1];
+      if (upto >= want && upto - own_sum[tid] < want) {      // one thread
+        found[0] = 255 - tid;
+        found[1] = upto - own_sum[tid];
+        found[2] = upto;
+      }
+    }
+    __syncthreads();
+    least |= static_cast<uint32_t>(found[0]) << shift;
+    above = found[1];
+    at_or_above = found[2];
   }
-  const int equal_wanted = want - above;     // of the tokens whose word is `prefix`, the first so many
-  // in order: which tokens stay, and where they go
-  int placed = 0, equal_seen = 0;            // before the current chunk, the same in all threads
-  for (int base = 0; base < length; base += CHOOSE_THREADS) {
-    const int i = base + tid;
-    bool stays = false, equal = false;
-    if (i < candidates && want > 0) {
-      const uint32_t w = word_at(i);
-      stays = w > prefix;
-      equal = w == prefix;
-    } else if (i >= candidates && i < length) {
-      stays = true;
+  // Words above `least` stay; of those equal to it the first so many (all, if the search ended with those wanted).
+  const int equal_wanted = at_or_above > want ? want - above : 0x7fffffff;
+
+  const uint64_t before = (1ull << lane) - 1;
+  int placed = 0, equal_seen = 0;
+  for (int base = 0; base < length; base += R * CHOOSE_THREADS) {      // R rounds at a time; the first from registers
+    if (base > 0) read_words(base, word);
+    if (equal_wanted != 0x7fffffff) {      // ties: which of the equal ones are among the first
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint64_t mask = __ballot(word[r] == least);
+        if (lane == 0) round_counts[r * CHOOSE_WAVES + wave] = __popcll(mask);
+      }
+      __syncthreads();
+      const int total = scan_counts(round_counts, R * CHOOSE_WAVES, wave_counts[0]);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const bool equal = word[r] == least;
+        const uint64_t mask = __ballot(equal);
+        // what does not stay becomes 0
+        if (equal && equal_seen + round_counts[r * CHOOSE_WAVES + wave] + __popcll(mask & before) >= equal_wanted) word[r] = 0;
+      }
+      equal_seen += total;
+      __syncthreads();
     }
-    const uint64_t equal_mask = __ballot(equal);
-    const uint64_t before = (1ull << lane) - 1;
-    if (lane == 0) wave_counts[0][wave] = __popcll(equal_mask);
+    auto stays = [&](int r) {
+      const int i = base + r * CHOOSE_THREADS + tid;
+      return (want > 0 && i < candidates && word[r] >= least && word[r] != 0) || (i >= candidates && i < length);
+    };
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const uint64_t mask = __ballot(stays(r));
+      if (lane == 0) round_counts[r * CHOOSE_WAVES + wave] = __popcll(mask);
+    }
     __syncthreads();
-    int equal_rank = equal_seen + __popcll(equal_mask & before), equal_total = 0;
-    for (int w = 0; w < CHOOSE_THREADS / SE_WAVE; ++w) {
-      if (w < wave) equal_rank += wave_counts[0][w];
-      equal_total += wave_counts[0][w];
+    const int total = scan_counts(round_counts, R * CHOOSE_WAVES, wave_counts[1]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool mine = stays(r);
+      const uint64_t mask = __ballot(mine);
+      const int rank = placed + round_counts[r * CHOOSE_WAVES + wave] + __popcll(mask & before);
+      if (mine && rank < keep) dst[rank] = base + r * CHOOSE_THREADS + tid;
     }
-    if (equal && equal_rank < equal_wanted) stays = true;
-    const uint64_t stay_mask = __ballot(stays);
-    if (lane == 0) wave_counts[1][wave] = __popcll(stay_mask);
-    __syncthreads();
-    int rank = placed + __popcll(stay_mask & before), total = 0;
-    for (int w = 0; w < CHOOSE_THREADS / SE_WAVE; ++w) {
-      if (w < wave) rank += wave_counts[1][w];
-      total += wave_counts[1][w];
-    }
-    if (stays && rank < keep) dst[rank] = i;
     placed += total;
-    equal_seen += equal_total;
+    __syncthreads();
   }
 }
 
@@ -207,8 +298,13 @@ extern "C" int se_evict_tokens(void* cache, int kind, float* weights, const int3
   if (recent < 0 || recent > keep || kv_heads <= 0 || kv_heads > 65535 || items > 32767) return SE_ERR_SHAPE;
   if (page_size <= 0 || page_size % 8 || page_size > 4096 || head_dim <= 0 || head_dim % 8) return SE_ERR_SHAPE;
   if (kind == 2 && (head_dim % 32 || page_size % 32)) return SE_ERR_SHAPE;
-  choose_tokens_kernel<<<dim3(kv_heads, items), CHOOSE_THREADS, 0, stream>>>(
-      weights, block_table, bt_stride, lengths, longest, kv_heads, page_size, keep, recent, kept);
+#define SE_CHOOSE(R)                                                              \
+  choose_tokens_kernel<R><<<dim3(kv_heads, items), CHOOSE_THREADS, 0, stream>>>( \
+      weights, block_table, bt_stride, lengths, longest, kv_heads, page_size, keep, recent, kept)
+  if (longest <= 4 * CHOOSE_THREADS) SE_CHOOSE(4);
+  else if (longest <= 16 * CHOOSE_THREADS) SE_CHOOSE(16);
+  else SE_CHOOSE(32);      // more than 32768 tokens: the rest is read again in every pass
+#undef SE_CHOOSE
   SE_CHECK_LAUNCH();
   const dim3 grid((keep + page_size - 1) / page_size, kv_heads, items * 2);
   const size_t shared = static_cast<size_t>(page_size) * 2 * sizeof(int);

@@ -113,9 +113,11 @@ _SIGNATURES = {
     },
     "attention_weights": {
         # q, q_stride, cache, kind, block_table, bt_stride, item_meta, items, longest, most_new, lse, previous, out,
-        # heads, kv_heads, head_dim, page_size, scale, window, dtype, stream
+        # heads, kv_heads, head_dim, page_size, scale, window, dtype, workspace, stream
         "se_attention_weights": [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_void_p,
-                                 c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
+                                 c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p],
+        # items, longest, most_new, heads, kv_heads, head_dim, dtype
+        "se_attention_weights_splits": [c_int] * 7,
     },
     "evict": {
         # cache, kind, weights, block_table, bt_stride, lengths, items, longest, new_table, new_stride, keep, recent,
@@ -558,10 +560,14 @@ class HipKernels:
             return
         items, longest, most_new, item_meta = self._items(meta, tokens, page)
         _same_device(q, cache, lse, out, previous, meta.block_table, item_meta)
+        # sums of several blocks for the same keys (many rows) meet in a workspace of this call's own
+        splits = _fn.get("attention_weights", "se_attention_weights_splits")(items, longest, most_new, heads, kv_heads,
+                                                                             head_dim, _code(q.dtype))
+        workspace = (torch.empty(splits, items, kv_heads, longest, dtype=torch.float32, device=q.device) if splits > 1 else None)
         _check(_fn.get("attention_weights", "se_attention_weights")(
             _ptr(q), q.stride(0), _ptr(cache), self._CACHE_KINDS[cache.dtype], _ptr(meta.block_table),
             meta.block_table.stride(0), _ptr(item_meta), items, longest, most_new, _ptr(lse), _ptr(previous), _ptr(out), heads, kv_heads,
-            head_dim, page, float(scale), int(window or 0), _code(q.dtype), _stream()), "attention_weights")
+            head_dim, page, float(scale), int(window or 0), _code(q.dtype), _ptr(workspace), _stream()), "attention_weights")
 
     def _items(self, meta, tokens: int, page: int):
         """(number of items, longest context, most new tokens, int32 ``[3, items]`` on the device) of a step, checked."""

@@ -561,6 +561,8 @@ inline float emu_max3_bare(float a, float b, float c) { return fmaxf(fmaxf(a, b)
 #define __builtin_amdgcn_permlane16_swap emu_permlane16_swap
 #define __builtin_amdgcn_permlane32_swap emu_permlane32_swap
 #define __builtin_amdgcn_readfirstlane(x) (x)      /* the kernels use it on wave-uniform values only */
+#define __builtin_amdgcn_readlane(x, lane) __shfl(x, lane, 64)
+#define __builtin_amdgcn_wave_barrier() ((void)emu_ballot_w64(true))     // the wavefront's lanes meet
 #define __builtin_amdgcn_ballot_w64 emu_ballot_w64
 #define __builtin_amdgcn_exp2f exp2f
 #define __log2f log2f

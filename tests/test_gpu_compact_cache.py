@@ -215,6 +215,8 @@ ATTEND = [  # heads, kv_heads, head_dim, page, contexts, new tokens, window
     (12, 2, 64, 32, [50, 61, 9], [40, 1, 9], 0),           # a prompt portion beside decoded tokens
     (12, 1, 128, 64, [150, 40], [70, 40], 0),
     (12, 1, 64, 32, [200, 40], [70, 1], 45),
+    (16, 1, 64, 32, [600, 70], [80, 1], 0),                # rows of the same keys in several blocks
+    (16, 1, 128, 32, [200], [80], 60),
 ]
 
 
@@ -347,6 +349,8 @@ EVICT = [  # kv_heads, head_dim, page, lengths, keep, recent
     (3, 96, 32, [100], 40, 40),
     (2, 64, 32, [65, 64, 63, 31], 64, 1),
     (1, 64, 96, [1500, 700], 100, 13),       # more than one round of the block
+    (2, 32, 64, [5000, 4097], 4000, 100),    # more than a thread's registers at the first size
+    (1, 32, 128, [60000, 20000, 49153], 5000, 0),    # more than the largest size holds
 ]
 
 
@@ -367,6 +371,7 @@ def evict_case(kind, dtype, kv, d, page, lengths, keep, seed=0):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kv,d,page,lengths,keep,recent", EVICT)
 def test_eviction(hip, dtype, kind, kv, d, page, lengths, keep, recent):
+    emulator_skips(sum(lengths) * kv * 1e4, 1e8)
     meta, cache, layer, weights, new_table = evict_case(kind, dtype, kv, d, page, lengths, keep)
     if kind == "own" and dtype == torch.float32:      # any float has a place in the order
         weights[0, 0, :4] = torch.tensor([float("inf"), float("nan"), -0.0, -1.0])
