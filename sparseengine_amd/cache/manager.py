@@ -21,6 +21,7 @@ import numpy as np
 import torch
 
 from ..parts.base import PagedKVRequest, StateRequest
+from .layout import fp4_row_bytes
 from .page_pool import OutOfPages, PageOwnershipError, PagePool
 
 
@@ -49,6 +50,12 @@ class KVGroup:
         return len(self.positions) * 2 * r.kv_heads * self.page_size * r.head_dim * itemsize
 
 
+def bytes_per_token(request: PagedKVRequest, dtype: torch.dtype) -> int:
+    """What one token of a position's cache takes; ``dtype`` uint8: in 4 bits."""
+    row = fp4_row_bytes(request.head_dim) if dtype == torch.uint8 else request.head_dim * torch.empty((), dtype=dtype).element_size()
+    return 2 * request.kv_heads * row
+
+
 @dataclass
 class StepAllocation:
     """What an ``append`` decided: for every group the slot of every new token, in item order."""
@@ -58,17 +65,19 @@ class StepAllocation:
 class CacheManager:
     def __init__(self, requests: dict[int, object], *, max_rows: int, max_model_len: int,
                  page_size: int, num_pages: int | dict | None = None, num_tokens: int | None = None,
-                 dtype: torch.dtype, device, allocate_tensors: bool = True):
+                 dtype: torch.dtype, device, allocate_tensors: bool = True, kv_dtype: torch.dtype | None = None):
         """``requests``: schedule position -> PagedKVRequest | StateRequest (positions that read
         another position's cache are not listed).  ``page_size``: tokens per page of the groups whose
         request names none.  The pools' sizes: ``num_tokens`` (every group gets the pages that hold so
-        many tokens) or ``num_pages`` (an int for all groups or {group index: pages})."""
+        many tokens) or ``num_pages`` (an int for all groups or {group index: pages}).  ``kv_dtype``: the
+        layers' type (None: ``dtype``); uint8 keeps keys and values in 4 bits (cache/layout.py)."""
         if page_size <= 0 or max_rows <= 0 or max_model_len <= 0:
             raise ValueError("page_size, max_rows and max_model_len must be positive")
         self.page_size = int(page_size)          # the default; a group's own is ``group.page_size``
         self.max_rows = int(max_rows)
         self.max_model_len = int(max_model_len)
         self.dtype, self.device = dtype, device
+        self.kv_dtype = kv_dtype or dtype
 
         by_geometry: dict[PagedKVRequest, list[int]] = {}
         self.state_positions: dict[int, StateRequest] = {}
@@ -86,6 +95,9 @@ class CacheManager:
             if ps <= 0 or ps % 8:
                 raise ValueError(f"a cache page holds a multiple of 8 tokens (it keeps its elements in groups of "
                                  f"eight, cache/layout.py), got {ps}")
+            if self.kv_dtype == torch.uint8 and (ps % 32 or req.head_dim % 32):
+                raise ValueError(f"a cache in 4 bits takes pages and head sizes in steps of 32, got pages of {ps} tokens and "
+                                 f"head_dim {req.head_dim}")
             if num_tokens is not None:
                 pages = max(1, -(-int(num_tokens) // ps))      # a last page may be partly beyond the count
             else:
@@ -97,8 +109,8 @@ class CacheManager:
                             np.zeros(self.max_rows, dtype=np.int64))
             if allocate_tensors:
                 for position in positions:
-                    group.layers[position] = torch.zeros(
-                        int(pages), 2, req.kv_heads, ps, req.head_dim, dtype=dtype, device=device)
+                    row = fp4_row_bytes(req.head_dim) if self.kv_dtype == torch.uint8 else req.head_dim
+                    group.layers[position] = torch.zeros(int(pages), 2, req.kv_heads, ps, row, dtype=self.kv_dtype, device=device)
             self.groups.append(group)
             for position in positions:
                 self.group_of_position[position] = index
@@ -110,7 +122,8 @@ class CacheManager:
                 for name, shape, dt in req.tensors} if allocate_tensors else {}
 
         self._no_window = all(group.window is None for group in self.groups)
-        self.row_len = np.zeros(self.max_rows, dtype=np.int64)
+        self.row_len = np.zeros(self.max_rows, dtype=np.int64)          # cached tokens
+        self.row_dropped = np.zeros(self.max_rows, dtype=np.int64)      # tokens evicted: the next position is their sum
         self.row_owner: list[object | None] = [None] * self.max_rows
         self._free_rows = deque(range(self.max_rows))
         self._row_of: dict[object, int] = {}
@@ -136,6 +149,7 @@ class CacheManager:
         self._row_of[request_id] = row
         self.row_owner[row] = request_id
         self.row_len[row] = 0
+        self.row_dropped[row] = 0
         for group in self.groups:
             group.first_live[row] = 0
         for tensors in self.state.values():
@@ -155,6 +169,7 @@ class CacheManager:
             group.table[row, :] = -1
             group.first_live[row] = 0
         self.row_len[row] = 0
+        self.row_dropped[row] = 0
         self.row_owner[row] = None
         self._free_rows.append(row)
 
@@ -194,7 +209,7 @@ class CacheManager:
                 need[gi] += pages
         free = self.free_pages()
         return all(need[gi] <= free[gi] for gi in need) and all(
-            self.row_len[row] + n <= self.max_model_len for row, n in items)
+            self.row_len[row] + self.row_dropped[row] + n <= self.max_model_len for row, n in items)
 
     # ------------------------------------------------------------------ the append of a step
     def append(self, items) -> StepAllocation:
@@ -212,8 +227,8 @@ class CacheManager:
                 raise PageOwnershipError(f"row {row} is not held by a request")
             if n <= 0:
                 raise ValueError("an item must bring at least one token")
-            if self.row_len[row] + n > self.max_model_len:
-                raise ValueError(f"row {row}: {self.row_len[row]} + {n} tokens exceed max_model_len "
+            if self.row_len[row] + self.row_dropped[row] + n > self.max_model_len:
+                raise ValueError(f"row {row}: {self.row_len[row] + self.row_dropped[row]} + {n} tokens exceed max_model_len "
                                  f"{self.max_model_len}")
         if not self.can_append(items):
             raise OutOfPages(f"step of {sum(n for _, n in items)} tokens does not fit: free pages "
@@ -253,8 +268,8 @@ class CacheManager:
         for row in rows:
             if self.row_owner[row] is None:
                 raise PageOwnershipError(f"row {row} is not held by a request")
-            if self.row_len[row] + 1 > limit:
-                raise ValueError(f"row {row}: {self.row_len[row]} + 1 tokens exceed max_model_len {limit}")
+            if self.row_len[row] + self.row_dropped[row] + 1 > limit:
+                raise ValueError(f"row {row}: {self.row_len[row] + self.row_dropped[row]} + 1 tokens exceed max_model_len {limit}")
         index = np.asarray(rows, dtype=np.int64)
         lengths = self.row_len[index]
         fresh = []                               # per group: which items start a new page
@@ -286,6 +301,33 @@ class CacheManager:
                 group.pool.release(group.table[row, first:have_until].tolist(), row)
                 group.table[row, first:have_until] = -1
         self.row_len[row] = length
+
+    # ------------------------------------------------------------------ letting tokens go
+    def begin_eviction(self, rows, keep: int) -> dict[int, np.ndarray]:
+        """Fresh pages for ``keep`` tokens of every listed row: group index -> int32 ``[rows, ceil(keep / page_size)]``.
+        They belong to the rows, beside their old ones, until ``finish_eviction``; all or nothing."""
+        for group in self.groups:
+            if group.window is not None:
+                raise ValueError("a windowed cache group gives its tokens back by itself")
+            if len(rows) * -(-keep // group.page_size) > group.pool.free_count:
+                raise OutOfPages(f"eviction of {len(rows)} rows to {keep} tokens: free pages {self.free_pages()}")
+        for row in rows:
+            if self.row_owner[row] is None or self.row_len[row] < keep:
+                raise ValueError(f"row {row} holds {self.row_len[row]} tokens: it cannot keep {keep}")
+        return {group.index: np.asarray([group.pool.allocate(-(-keep // group.page_size), row) for row in rows], dtype=np.int32)
+                for group in self.groups}
+
+    def finish_eviction(self, rows, keep: int, tables: dict[int, np.ndarray]) -> None:
+        """The rows' tokens have been moved to the pages of ``tables``: their old pages return to the pool."""
+        for group in self.groups:
+            for row, pages in zip(rows, tables[group.index]):
+                held = group.table[row]
+                group.pool.release(held[held >= 0].tolist(), row)
+                group.table[row, :] = -1
+                group.table[row, :len(pages)] = pages
+        for row in rows:
+            self.row_dropped[row] += self.row_len[row] - keep
+            self.row_len[row] = keep
 
     # ------------------------------------------------------------------ views for the step
     def kv_layer(self, position: int) -> torch.Tensor:

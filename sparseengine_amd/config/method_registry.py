@@ -1,7 +1,8 @@
 """Registry of sparse-attention methods and their prefill policies.
 
-Only the dense method is registered: ``""`` (alias ``"vanilla"``) with the ``all_chunked`` prefill
-policy and the paged cache manager.  A method brings three things under its name: the runtime with
+Registered are the dense method, ``""`` (alias ``"vanilla"``), and ``"accumulated_weight"``, which lets the tokens
+go that have gathered the least attention (engine/eviction.py); both with the ``all_chunked`` prefill policy and the
+paged cache manager.  A method brings three things under its name: the runtime with
 its step hooks, its prefill policy and the class of its cache manager, which the model runner builds
 in place of the paged one (reference: method_registry.py:19-36,508-525,646-665; the cache-manager
 factory by method engine/cache_manager/base.py:537-647; the pass-through runtime
@@ -29,15 +30,42 @@ class MethodRuntime:
     ``finish_step(fb)``            after the last layer, before logits leave the step;
     ``extra_pages(row, new_tokens)`` pages per group index the method needs for itself on top of
                                    what the cache manager counts for an append (temporary slots);
-                                   the scheduler's capacity questions add them.
+                                   the scheduler's capacity questions add them;
+    ``tokens_taken(length, n)``    how many more tokens of cache a request that holds ``length`` takes at most
+                                   while ``n`` are added to it, in steps' portions (the dense method: n);
+    ``reserved_pages()``           {group index: pages} that no request may take;
+    ``kernel_libraries``           the kernel libraries it calls;
+    ``configure(config)``          once, before the runner is built, with the runtime configuration;
+    ``bytes_per_token(request)``   device memory the method keeps per cached token and position beside the cache;
+    ``attended(position, fb, q, cache, meta, lse, scale, window)``
+                                   only with ``wants_attention``: after the attention of a position that writes
+                                   its own cache, with the step's queries and every row's logarithm of its sum of
+                                   exponentials.
 
     (Reference: engine/sparse_methods/base.py:324-500 prepare_step / build_*_selection /
     on_attention_end / finish_step; engine/cache_manager/base.py:1335-1361 the cache-side hooks.)
     """
     name = ""
+    wants_attention = False
+    kernel_libraries: tuple[str, ...] = ()
+
+    def configure(self, config) -> None:
+        pass
 
     def bind(self, cache) -> None:
         self.cache = cache
+
+    def attended(self, position: int, fb, q, cache, meta, lse, scale: float, window: int) -> None:
+        pass
+
+    def tokens_taken(self, length: int, new_tokens: int) -> int:
+        return new_tokens
+
+    def reserved_pages(self) -> dict[int, int]:
+        return {}
+
+    def bytes_per_token(self, request) -> int:
+        return 0
 
     def prepare_step(self, fb) -> None:
         pass
@@ -109,4 +137,10 @@ def resolve_prefill_schedule_policy(method: str, requested: str = PREFILL_POLICY
                      f"{method or 'vanilla'!r}, whose policy is {default!r}")
 
 
+def _accumulated_weight():
+    from ..engine.eviction import AccumulatedWeightMethod
+    return AccumulatedWeightMethod()
+
+
 register_method("", PassThroughMethod, "all_chunked")
+register_method("accumulated_weight", _accumulated_weight, "all_chunked")

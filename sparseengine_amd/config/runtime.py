@@ -1,7 +1,8 @@
 """The typed runtime configuration.  Its fields are exactly the keyword arguments of
 ``LLM(model, **kwargs)``; an unknown keyword is an error.  Names and meanings are the reference's
 where it has them (configs/runtime.py:51-105, configs/groups.py, configs/scheduling.py:15-186);
-``dtype``, ``kv_page_size``, ``sampler_seed`` and ``tiny_random_on_device`` are this engine's own.
+``dtype``, ``kv_page_size``, ``kv_cache_dtype``, ``eviction_budget``, ``eviction_recent``, ``sampler_seed`` and
+``tiny_random_on_device`` are this engine's own.
 """
 from __future__ import annotations
 
@@ -45,11 +46,26 @@ class Config:
     throughput_log_interval_s: float = 0.0
     dtype: str = "bfloat16"                       # "bfloat16" | "float32"
     kv_page_size: int = 64
+    kv_cache_dtype: str = AUTO                    # "auto": dtype; "fp4": keys and values in 4 bits (cache/layout.py)
+    eviction_budget: int = 0                      # sparse_method "accumulated_weight": cached tokens a request keeps
+    eviction_recent: int = -1                     # of which its last so many (-1: a quarter)
     sampler_seed: int = 0
     # derived, not keyword arguments
     raw_model_config: dict = field(default=None, init=False, repr=False)
     model_config: object = field(default=None, init=False, repr=False)
     architecture: object = field(default=None, init=False, repr=False)
+
+    def _check_eviction(self) -> None:
+        if self.sparse_method != "accumulated_weight":
+            if self.eviction_budget or self.eviction_recent != -1:
+                raise ValueError("eviction_budget and eviction_recent belong to sparse_method 'accumulated_weight'")
+            return
+        if self.eviction_budget < 1:
+            raise ValueError("sparse_method 'accumulated_weight' needs eviction_budget, the number of cached tokens a request keeps")
+        if self.eviction_recent == -1:
+            self.eviction_recent = self.eviction_budget // 4
+        if not 0 <= self.eviction_recent <= self.eviction_budget:
+            raise ValueError(f"eviction_recent must be between 0 and eviction_budget, got {self.eviction_recent}")
 
     @classmethod
     def keyword_names(cls) -> set[str]:
@@ -72,6 +88,11 @@ class Config:
             raise ValueError(f"dtype must be 'bfloat16' or 'float32', got {self.dtype!r}")
         if self.kv_page_size <= 0 or self.kv_page_size % 8:
             raise ValueError(f"kv_page_size must be a positive multiple of 8, got {self.kv_page_size}")
+        if self.kv_cache_dtype not in (AUTO, "fp4"):
+            raise ValueError(f"kv_cache_dtype must be 'auto' or 'fp4', got {self.kv_cache_dtype!r}")
+        if self.kv_cache_dtype == "fp4" and self.kv_page_size % 32:
+            raise ValueError(f"a cache in 4 bits has pages in steps of 32 tokens, got kv_page_size {self.kv_page_size}")
+        self._check_eviction()
         if not 0.0 < self.gpu_memory_utilization <= 1.0:
             raise ValueError("gpu_memory_utilization must be in (0, 1]")
         if self.max_num_seqs_in_batch <= 0:

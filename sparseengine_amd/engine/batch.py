@@ -15,7 +15,8 @@ import numpy as np
 import torch
 
 from ..cache.manager import CacheManager
-from ..kernels.attention_work import DeviceAttentionWork, build_attention_work
+from ..kernels.attention_work import (FP4_HEAD_DIMS, DeviceAttentionWork, build_attention_work, build_fp4_attention_work,
+                                      fp4_unpack_list)
 from ..parts.base import StepScratch
 
 
@@ -31,7 +32,8 @@ class GroupMeta:
     """Per cache group: where every token of the step lives and how to find its request's pages."""
     block_table: torch.Tensor      # int32 [items, pages]: compact table of the step's requests
     token_row: torch.Tensor        # int32 [T] index of the token's item = row of block_table
-    positions: torch.Tensor        # int32 [T]
+    positions: torch.Tensor        # int32 [T] index of the token's own key among its request's cached tokens (the
+                                   # token's position in the sequence, unless the request has let tokens go)
     slots: torch.Tensor            # int32 [T] page * page_size + offset of the token's own key
     page_size: int
     block_table_host: np.ndarray = None   # block_table on the host (for checks before a launch)
@@ -57,7 +59,7 @@ class ForwardBatch:
         self.num_tokens = 0
         self.num_items = 0
         self.token_ids = None          # int32 [T]
-        self.positions = None          # int32 [T]
+        self.positions = None          # int32 [T]: the tokens' positions in their sequences
         self.token_item = None         # int32 [T]
         self.item_rows = None          # int32 [items]: the cache row (state slot) of every item
         self.item_rows_host = None
@@ -166,11 +168,13 @@ class BatchBuilder:
             for it in items:
                 if it.want and any(w != 0 for w in it.want):
                     raise ValueError("a wanted place lies outside the item's tokens")
-            positions = cache.row_len[rows].astype(np.int32)
+            places = cache.row_len[rows].astype(np.int32)
+            dropped = cache.row_dropped[rows]
             allocation = cache.append([(it.row, 1) for it in items])   # all or nothing
             q_start = token_item = np.arange(B, dtype=np.int32)
             q_len = np.ones(B, dtype=np.int32)
-            ctx_len = positions + 1
+            ctx_len = places + 1
+            positions = places + dropped.astype(np.int32) if dropped.any() else places
             want = np.asarray([i for i, it in enumerate(items) for _ in it.want], dtype=np.int32)
         else:
             for it in items:
@@ -188,7 +192,9 @@ class BatchBuilder:
             q_len = np.asarray(lengths, dtype=np.int32)
             ctx_len = np.asarray([s + n for s, n in zip(starts, lengths)], dtype=np.int32)
             token_ids = np.concatenate([np.asarray(it.tokens, dtype=np.int32) for it in items])
-            positions = np.concatenate([np.arange(s, s + n, dtype=np.int32) for s, n in zip(starts, lengths)])
+            places = np.concatenate([np.arange(s, s + n, dtype=np.int32) for s, n in zip(starts, lengths)])
+            dropped = cache.row_dropped[[it.row for it in items]]
+            positions = places + np.repeat(dropped, lengths).astype(np.int32) if dropped.any() else places
             token_item = np.repeat(np.arange(B, dtype=np.int32), lengths)
             want = np.asarray([q_start[i] + w for i, it in enumerate(items) for w in it.want], dtype=np.int32)
             rows = np.asarray([it.row for it in items], dtype=np.int32)
@@ -202,14 +208,25 @@ class BatchBuilder:
         parts = [token_ids, positions, token_item, rows, item_meta_host.reshape(-1), want]
         for group in cache.groups:
             parts += [allocation.slots[group.index], tables[group.index].reshape(-1)]
-        works = []
+        places_at = None
+        if places is not positions:
+            places_at = len(parts)
+            parts.append(places)
+        works, lists = [], []
         if self.attention_shapes:
+            fp4 = cache.kv_dtype == torch.uint8
             for group in cache.groups:
+                head_dim = group.request.head_dim
+                direct = fp4 and self.dtype == torch.bfloat16 and head_dim in FP4_HEAD_DIMS
                 for ratio, window in sorted(self.attention_shapes.get(group.index, ())):
-                    work = build_attention_work(q_len, ctx_len, ratio, group.request.kv_heads, window,
-                                                head_dim=group.request.head_dim)
-                    works.append((group.index, (ratio, window), work, len(parts)))
+                    build = build_fp4_attention_work if direct else build_attention_work
+                    work = build(q_len, ctx_len, ratio, group.request.kv_heads, window, head_dim=head_dim)
+                    works.append((group.index, (ratio, window, "fp4") if direct else (ratio, window), work, len(parts)))
                     parts += [work.units.reshape(-1), work.tasks.reshape(-1), work.block_units.reshape(-1)]
+                    if fp4 and (not direct or len(work.block_units)):
+                        pairs, table = fp4_unpack_list(q_len, ctx_len, ratio, head_dim, group.page_size, window, direct)
+                        lists.append((group.index, ("unpack", ratio, head_dim, group.page_size, window, direct), pairs, table, len(parts)))
+                        parts += [pairs.reshape(-1), table.reshape(-1)]
         # every part starts on a 16-byte boundary: kernels read records of four ints at once
         total = sum(-(-p.size // 4) * 4 for p in parts)
         if self._copied is not None:
@@ -241,7 +258,7 @@ class BatchBuilder:
             fb.groups[group.index] = GroupMeta(
                 block_table=view(6 + 2 * gi + 1, tables[group.index].shape),
                 block_table_host=tables[group.index],
-                token_row=fb.token_item, positions=fb.positions, slots=view(6 + 2 * gi),
+                token_row=fb.token_item, positions=fb.positions if places_at is None else view(places_at), slots=view(6 + 2 * gi),
                 page_size=group.page_size, item_q_start=q_start, item_q_len=q_len,
                 item_ctx_len=ctx_len, item_meta=item_meta, max_ctx_len=int(ctx_len.max()),
                 max_q_len=int(q_len.max()))
@@ -250,4 +267,6 @@ class BatchBuilder:
                 view(at, work.units.shape), work.units.shape[0], view(at + 1, work.tasks.shape),
                 work.tasks.shape[0], work.num_slots, view(at + 2, work.block_units.shape),
                 work.block_units.shape[0], work.tiles_per_block)
+        for group_index, key, pairs, table, at in lists:
+            fb.groups[group_index].work[key] = (view(at, pairs.shape), view(at + 1, table.shape))
         return fb

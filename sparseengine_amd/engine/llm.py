@@ -29,12 +29,13 @@ class CacheOracle(MemoryOracle):
     def __init__(self, cache, method=None):
         self.cache = cache
         self.method = method
+        self._reserved = {} if method is None else method.reserved_pages()
 
     def free_tokens(self):
-        return min((g.pool.free_count * g.page_size for g in self.cache.groups), default=1 << 40)
+        return min(((g.pool.free_count - self._reserved.get(g.index, 0)) * g.page_size for g in self.cache.groups), default=1 << 40)
 
     def total_tokens(self):
-        return min((g.pool.num_pages * g.page_size for g in self.cache.groups), default=1 << 40)
+        return min(((g.pool.num_pages - self._reserved.get(g.index, 0)) * g.page_size for g in self.cache.groups), default=1 << 40)
 
     def free_rows(self):
         return self.cache.num_free_rows
@@ -46,8 +47,11 @@ class CacheOracle(MemoryOracle):
         sizes = {g.index: g.page_size for g in self.cache.groups}
         return max((n * sizes[group] for group, n in pages.items()), default=0)
 
+    def _taken(self, length: int, new_tokens: int) -> int:
+        return new_tokens if self.method is None else self.method.tokens_taken(length, new_tokens)
+
     def cost_of_new(self, tokens):
-        return self._cost(self.cache.pages_for_tokens(tokens), None, tokens)
+        return self._cost(self.cache.pages_for_tokens(self._taken(0, tokens)), None, tokens)
 
     def cost_to_append(self, seq_id, new_tokens):
         if new_tokens <= 0:
@@ -55,7 +59,8 @@ class CacheOracle(MemoryOracle):
         if not self.cache.has_row(seq_id):
             return self.cost_of_new(new_tokens)
         row = self.cache.row_of(seq_id)
-        return self._cost(self.cache.pages_needed(row, new_tokens), row, new_tokens)
+        taken = self._taken(int(self.cache.row_len[row]), new_tokens)
+        return self._cost(self.cache.pages_needed(row, taken), row, new_tokens)
 
     def tokens_that_fit(self, seq_id, room):
         length = int(self.cache.row_len[self.cache.row_of(seq_id)]) if self.cache.has_row(seq_id) else 0
@@ -140,11 +145,12 @@ class LLM:
         self.config = config = Config.from_kwargs(model, **kwargs)
         binding = resolve_method(config.sparse_method)
         self.method = binding.runtime_factory()
+        self.method.configure(config)
         cache_tokens = config.num_kvcache_slots
         common = dict(dtype=config.dtype, device=device, kv_page_size=config.kv_page_size,
                       max_num_seqs=config.max_num_seqs_in_gpu, max_model_len=config.max_model_len,
                       mlp_chunk_size=config.mlp_chunk_size, kernels=kernels, method=self.method,
-                      cache_manager_cls=binding.cache_manager(),
+                      cache_manager_cls=binding.cache_manager(), kv_cache_dtype=config.kv_cache_dtype,
                       validate_runtime_invariants=config.validate_runtime_invariants)
         if config.tiny_random:
             self.runner = ModelRunner.from_random(config.raw_model_config, seed=config.tiny_random_seed,

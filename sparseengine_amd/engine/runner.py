@@ -12,7 +12,7 @@ from dataclasses import dataclass, field
 
 import torch
 
-from ..cache.manager import CacheManager
+from ..cache.manager import CacheManager, bytes_per_token
 from ..config.registry import Architecture, read_config_json, resolve_architecture
 from ..weights import loader as weight_loader
 from ..weights import random_weights
@@ -71,13 +71,20 @@ class ModelRunner:
     def __init__(self, arch: Architecture, cfg, params_factory, *, dtype, device="cuda", kv_page_size=64,
                  num_kvcache_tokens: int | None = None, max_num_seqs: int = 8, max_model_len: int | None = None,
                  mlp_chunk_size: int = 16384, kernels=None, gpu_memory_utilization: float = 0.9, method=None,
-                 cache_manager_cls=None, validate_runtime_invariants: bool = False):
-        """``method`` / ``cache_manager_cls``: the sparse method's runtime and the class of its cache manager
+                 cache_manager_cls=None, validate_runtime_invariants: bool = False, kv_cache_dtype: str = "auto"):
+        """``kv_cache_dtype``: "auto" (``dtype``) or "fp4" (keys and values in 4 bits).  ``method`` / ``cache_manager_cls``: the sparse method's runtime and the class of its cache manager
         (config/method_registry.py); absent: the dense method on the paged cache manager.
         ``validate_runtime_invariants``: before every attention launch the host checks that each block-table
         entry the launch will read names a page of the pool."""
         self.arch, self.model_config = arch, cfg
         self.dtype = resolve_dtype(dtype)
+        if kv_cache_dtype not in ("auto", "fp4"):
+            raise ValueError(f"kv_cache_dtype must be 'auto' or 'fp4', got {kv_cache_dtype!r}")
+        self.kv_dtype = torch.uint8 if kv_cache_dtype == "fp4" else self.dtype
+        if method is None:
+            from ..config.method_registry import PassThroughMethod
+            method = PassThroughMethod()
+        self.method = method
         self.device = torch.device(device)
         require_true_float32()
         if kernels is None:
@@ -88,7 +95,7 @@ class ModelRunner:
         self.model = arch.make_model(self.spec, chunk_tokens=mlp_chunk_size)
         if getattr(kernels, "libraries", None):
             from ..kernels import library
-            library.ensure_built(sorted(self.model.all_kernel_libraries()))
+            library.ensure_built(sorted(self.model.all_kernel_libraries() | set(self.method.kernel_libraries)))
         self.max_model_len = int(max_model_len or self.spec.max_position)
         if self.max_model_len > self.spec.max_position:
             raise ValueError(f"max_model_len {self.max_model_len} exceeds the model's "
@@ -105,7 +112,8 @@ class ModelRunner:
         self.cache = (cache_manager_cls or CacheManager)(requests, max_rows=max_num_seqs,
                                                          max_model_len=self.max_model_len, page_size=self.kv_page_size,
                                                          num_tokens=int(num_kvcache_tokens), dtype=self.dtype,
-                                                         device=self.device)
+                                                         device=self.device,
+                                                         **({} if self.kv_dtype == self.dtype else {"kv_dtype": self.kv_dtype}))
         shapes = {}
         if getattr(kernels, "libraries", None):
             for position in requests:
@@ -114,10 +122,6 @@ class ModelRunner:
                     shapes.setdefault(self.cache.group_of_position[position], set()).add(key())
         self.builder = BatchBuilder(kernels, self.cache, self.dtype, self.device, self.spec.vocab_size,
                                     attention_shapes=shapes)
-        if method is None:
-            from ..config.method_registry import PassThroughMethod
-            method = PassThroughMethod()
-        self.method = method
         method.bind(self.cache)
         self.validate_runtime_invariants = bool(validate_runtime_invariants)
 
@@ -125,8 +129,7 @@ class ModelRunner:
         """Tokens of cache that fit the memory left after the weights: ``utilization`` of the card
         minus what is in use, capped by what ``max_num_seqs`` requests of full length could hold."""
         from ..parts.base import PagedKVRequest
-        itemsize = torch.empty((), dtype=self.dtype).element_size()
-        per_token = sum(2 * r.kv_heads * r.head_dim * itemsize for r in requests.values()
+        per_token = sum(bytes_per_token(r, self.kv_dtype) + self.method.bytes_per_token(r) for r in requests.values()
                         if isinstance(r, PagedKVRequest))
         cap = max_num_seqs * self.max_model_len
         if per_token == 0 or self.device.type != "cuda":

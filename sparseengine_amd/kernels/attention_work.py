@@ -137,6 +137,24 @@ def build_fp4_attention_work(q_len, ctx_len, group: int, kv_heads: int, window: 
     return build_attention_work(q_len, ctx_len, group, kv_heads, window, max(1, wanted - tiles), head_dim, FP4_MIN_SPLIT_KEYS)
 
 
+FP4_HEAD_DIMS = (64, 128, 256)      # head sizes that the 4-bit attention kernel is built for
+
+
+def fp4_unpack_list(q_len, ctx_len, group: int, head_dim: int, page: int, window: int, only_blocks: bool):
+    """Which pages of a 4-bit cache a step reads through unpacked copies (those of the block kernel's items, or of all):
+    int32 ``[n, 2]`` (item, column of the block table), and int32 ``[items, columns]`` where each lies among them."""
+    q_len, ctx_len = np.asarray(q_len, dtype=np.int64), np.asarray(ctx_len, dtype=np.int64)
+    chosen = items_in_blocks(q_len, group, head_dim) if only_blocks else np.ones(q_len.size, dtype=bool)
+    low = np.maximum(0, ctx_len - q_len - window + 1) if window else np.zeros_like(ctx_len)
+    first, until = low // page, -(-ctx_len // page)
+    column = np.arange(int(until.max()))[None, :]
+    read = (column >= first[:, None]) & (column < until[:, None]) & chosen[:, None]
+    pairs = np.ascontiguousarray(np.argwhere(read), dtype=np.int32)
+    table = np.zeros(read.shape, dtype=np.int32)
+    table[read] = np.arange(pairs.shape[0], dtype=np.int32)
+    return pairs, table
+
+
 def items_in_blocks(q_len, group: int, head_dim: int) -> np.ndarray:
     """Which items go to the block kernel: those with at least half a block of tiles."""
     tiles = (np.asarray(q_len, dtype=np.int64) * group + 15) // 16

@@ -13,6 +13,7 @@ import numpy as np
 import torch
 
 from . import library
+from .attention_work import FP4_HEAD_DIMS, fp4_unpack_list
 
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
 
@@ -464,8 +465,6 @@ class HipKernels:
             _ptr(cache), _ptr(pages), 0, None, pages.numel(), _ptr(out), cache.shape[2], page, out.shape[4],
             _code(out.dtype), _stream()), "unpack_cache")
 
-    FP4_HEAD_DIMS = (64, 128, 256)      # head sizes that the 4-bit attention kernel is built for
-
     def _paged_attention_fp4(self, q, cache, meta, out, scale, window, lse):
         """Attention over a 4-bit cache.  In bfloat16, at the head sizes its kernel takes, items of few rows (the
         work list's units) are read in 4 bits; the pages of items of many rows (its blocks: a page is then read
@@ -477,7 +476,7 @@ class HipKernels:
         if getattr(meta, "item_q_len", None) is None:
             raise ValueError("attention over a 4-bit cache needs the step's items (item_q_len, item_ctx_len)")
         _require(scale > 0, "attention over a 4-bit cache: scale must be positive")
-        direct = q.dtype == torch.bfloat16 and head_dim in self.FP4_HEAD_DIMS
+        direct = q.dtype == torch.bfloat16 and head_dim in FP4_HEAD_DIMS
         group = heads // kv_heads
         work = (self._attention_work(q, meta, heads, kv_heads, head_dim, window, fp4=direct)
                 if q.dtype == torch.bfloat16 else None)
@@ -506,16 +505,7 @@ class HipKernels:
         key = ("unpack", group, head_dim, page, window, only_blocks)
         if kept is not None and key in kept:
             return kept[key]
-        from .attention_work import items_in_blocks
-        q_len, ctx_len = np.asarray(meta.item_q_len, dtype=np.int64), np.asarray(meta.item_ctx_len, dtype=np.int64)
-        chosen = items_in_blocks(q_len, group, head_dim) if only_blocks else np.ones(q_len.size, dtype=bool)
-        low = np.maximum(0, ctx_len - q_len - window + 1) if window else np.zeros_like(ctx_len)
-        first, until = low // page, -(-ctx_len // page)
-        column = np.arange(int(until.max()))[None, :]
-        read = (column >= first[:, None]) & (column < until[:, None]) & chosen[:, None]
-        pairs = np.ascontiguousarray(np.argwhere(read), dtype=np.int32)
-        table = np.zeros(read.shape, dtype=np.int32)
-        table[read] = np.arange(pairs.shape[0], dtype=np.int32)
+        pairs, table = fp4_unpack_list(meta.item_q_len, meta.item_ctx_len, group, head_dim, page, window, only_blocks)
         device = meta.block_table.device
         made = (torch.from_numpy(pairs).to(device), torch.from_numpy(table).to(device))
         if kept is not None:

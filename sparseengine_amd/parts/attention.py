@@ -5,12 +5,14 @@ projection -> QK RMSNorm (optional: flat, over the whole q row and the whole k r
 per head with weights of one head's size, models/qwen3.py:116-118,151-153) -> rotation of
 the leading rotary dims of every head -> k (normed, rotated) and v written to this step's slots
 -> attention of the step's queries over everything the request has cached, its own tokens
-included -> output projection.  Norm, rotation and the cache write are one kernel when the position
+included -> output projection.  The cache may be in the engine's type or in 4 bits: the kernels see which.  Norm, rotation and the cache write are one kernel when the position
 part is a rotation by a table (``fused_rotation()`` hands the kernel its arguments); a position part
 that is something else returns None there and has ``apply(fb, q, k, positions)``, which changes
 ``q [T, heads, D]`` and ``k [T, kv_heads, D]`` in place between the norm and the cache write.
 """
 from __future__ import annotations
+
+import torch
 
 from ..config.specs import AttentionSpec
 from .base import MIXERS, POSITIONS, PagedKVRequest, ParamDecl, Part
@@ -18,7 +20,7 @@ from .linear import linear, prepare
 
 
 class GQAAttention(Part):
-    kernel_libraries = ("rope_kv", "attention_generic", "attention_mfma", "host_work")
+    kernel_libraries = ("rope_kv", "attention_generic", "attention_mfma", "host_work", "cache_fp4", "attention_fp4")
 
     def __init__(self, spec: AttentionSpec, hidden_size: int):
         if spec.num_kv_heads <= 0 or spec.num_heads % spec.num_kv_heads:
@@ -75,25 +77,30 @@ class GQAAttention(Part):
         per_head = s.qk_norm == "per_head"
         if rotation is not None:      # a rotation by a table: norm, rotation and cache write in one launch
             fb.kernels.qk_norm_rope_store(
-                qkv, meta.positions, rotation.table, p.get("q_norm"), p.get("k_norm"), s.qk_norm_eps,
+                qkv, fb.positions, rotation.table, p.get("q_norm"), p.get("k_norm"), s.qk_norm_eps,
                 s.num_heads, s.num_kv_heads, s.head_dim, rotation.rotary_dim, *store, meta.page_size,
                 pairing=rotation.pairing, per_head_norm=per_head)
         else:                         # the position part applies itself, between the norm and the cache write
             if "q_norm" in p:
-                fb.kernels.qk_norm_rope_store(qkv, meta.positions, None, p["q_norm"], p["k_norm"], s.qk_norm_eps,
+                fb.kernels.qk_norm_rope_store(qkv, fb.positions, None, p["q_norm"], p["k_norm"], s.qk_norm_eps,
                                               s.num_heads, s.num_kv_heads, s.head_dim, 0, None, None, meta.page_size,
                                               per_head_norm=per_head)
             k = qkv[:, self.q_width:self.q_width + self.kv_width].view(T, s.num_kv_heads, s.head_dim)
-            self.position.apply(fb, q, k, meta.positions)
+            self.position.apply(fb, q, k, fb.positions)
             if write_cache:
-                fb.kernels.qk_norm_rope_store(qkv, meta.positions, None, None, None, s.qk_norm_eps, s.num_heads,
+                fb.kernels.qk_norm_rope_store(qkv, fb.positions, None, None, None, s.qk_norm_eps, s.num_heads,
                                               s.num_kv_heads, s.head_dim, 0, *store, meta.page_size)
         attended = fb.buffer("attn.out", (T, self.q_width))
         method = getattr(fb, "method", None)
         visible = meta if method is None else method.select(cache_position, meta)     # what this layer may read
         if getattr(fb, "check_tables", False):
             fb.check_block_table(visible, s.window or 0, cache.shape[0], f"schedule position {cache_position}")
-        fb.kernels.paged_attention(q, cache, visible, attended, s.scale, s.window or 0)
+        if method is not None and method.wants_attention and write_cache:
+            lse = fb.buffer("attn.lse", (T, s.num_heads), torch.float32)
+            fb.kernels.paged_attention(q, cache, visible, attended, s.scale, s.window or 0, lse=lse)
+            method.attended(cache_position, fb, q, cache, visible, lse, s.scale, s.window or 0)
+        else:
+            fb.kernels.paged_attention(q, cache, visible, attended, s.scale, s.window or 0)
         if method is not None:
             method.after_attention(cache_position, fb)
         if fb.taps is not None:
