@@ -17,7 +17,13 @@
 // so that what one matrix-core operand load of sixteen lanes takes is one contiguous stretch.  A
 // token's slot is page * page_size + offset; negative slots are skipped.  page_size % 8 == 0 and
 // head_dim % 8 == 0.
+//
+// A layer in 4 bits (fp4.h) is written by the vector kernel too: the k and v it holds in registers become codes there
+// (FP4 below), in place of a second kernel that reads them back.
 #include "common.h"
+#include "fp4.h"
+
+#define WRITE_FP4 2      // write_kv: 0 no cache, 1 a cache in the storage type, 2 one in 4 bits
 
 // the storage value whose widening to float is `v`, bit for bit (NaN payloads included)
 template <typename T>
@@ -144,7 +150,7 @@ __global__ void qk_norm_rope_store_kernel(T* qkv, int64_t row_stride,
 // in shared memory in the storage type (only rotation partners and the value copy read them
 // there), and after the two reductions normalises and rotates its own vectors.  With few tokens
 // the block is 1024 threads wide and a thread has one or two vectors.
-template <typename T, typename W, int MAXV>
+template <typename T, typename W, int MAXV, bool FP4>
 __global__ void __launch_bounds__(1024)
 qk_norm_rope_store_vec_kernel(T* qkv, int64_t row_stride, const int32_t* __restrict__ positions,
                               const float* __restrict__ cos_sin, const W* __restrict__ q_weight,
@@ -286,13 +292,56 @@ qk_norm_rope_store_vec_kernel(T* qkv, int64_t row_stride, const int32_t* __restr
       outv.set(j, y);
     }
     *reinterpret_cast<raw_t*>(src + c0) = outv.v;
-    if (!is_q && k_dst >= 0) {
+    if constexpr (FP4) {
+      own[i].v = outv.v;
+    } else if (!is_q && k_dst >= 0) {
       const int head = local0 / head_dim;
       *reinterpret_cast<raw_t*>(cache + k_dst + static_cast<int64_t>(head) * page_size * head_dim +
                                 key_place(page_size, page_off, d0)) = outv.v;
     }
   }
 #undef QK_FETCH_TABLES
+  if constexpr (FP4) {
+    // A group of 32 dims lies in 32 / VN neighbouring lanes' vectors: its largest magnitude goes around those (as the
+    // bits of a float, whose order is that of the magnitudes, infinities and NaN above all), each lane makes its codes.
+    if (slot < 0) return;
+    uint8_t* out = reinterpret_cast<uint8_t*>(cache);
+    const int off = slot % page_size;
+#pragma unroll
+    for (int i = 0; i < MAXV; ++i) {
+      const int vi = threadIdx.x + i * threads;
+      const bool mine = vi >= qvec && vi < nvec;
+      const int which = vi >= qkvec, local0 = (vi - (which ? qkvec : qvec)) * VN;
+      const int head = local0 / head_dim, d0 = local0 % head_dim, group = d0 / FP4_GROUP;
+      uint32_t top = 0;
+      if (mine) {
+#pragma unroll
+        for (int j = 0; j < VN; ++j) top = max(top, __float_as_uint(own[i].get(j)) & 0x7fffffffu);
+      }
+#pragma unroll
+      for (int lanes = 1; lanes < FP4_GROUP / VN; lanes *= 2) top = max(top, __shfl_xor(top, lanes));
+      if (!mine) continue;
+      const int factor = fp4_factor_of(__uint_as_float(top));
+      const float inverse = factor == FP4_NAN ? 0.f : fp4_inverse(factor);
+      uint32_t word = 0;
+#pragma unroll
+      for (int j = 0; j < VN; ++j) word |= fp4_code(own[i].get(j) * inverse) << (4 * j);
+      uint8_t* part = out + ((static_cast<int64_t>(slot / page_size) * 2 + which) * kv_heads + head) * fp4_head_bytes(page_size, head_dim);
+      const int j0 = d0 % FP4_GROUP / 2;      // the byte of 16 that this vector's first two codes make
+      if (!which) {
+        uint8_t* at = part + fp4_key_code_at(page_size, off, group) + j0;
+        if constexpr (VN == 8) *reinterpret_cast<uint32_t*>(at) = word;
+        else *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(word);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VN / 2; ++j) part[fp4_value_code_at(head_dim, off, group, j0 + j)] = static_cast<uint8_t>(word >> (8 * j));
+      }
+      if (j0 == 0)
+        part[which ? fp4_value_factor_at(page_size, head_dim, off, group) : fp4_key_factor_at(page_size, head_dim, off, group)] =
+            static_cast<uint8_t>(factor);
+    }
+    return;
+  }
   if (v_dst >= 0) {   // values: a copy, bit for bit, to their place among the page's groups of eight keys
     const T* v = reinterpret_cast<const T*>(row_bytes) + q_width + k_width;
     for (int c = threadIdx.x; c < k_width; c += threads) {
@@ -302,15 +351,27 @@ qk_norm_rope_store_vec_kernel(T* qkv, int64_t row_stride, const int32_t* __restr
   }
 }
 
+template <typename T, typename W, int MAXV, bool FP4>
+static void launch_vec_to(int threads, size_t shmem, void* qkv, int64_t row_stride, const int32_t* positions,
+                          const float* cos_sin, const void* qw, const void* kw, float eps, int tokens,
+                          int heads, int kv_heads, int head_dim, int rotary_dim, void* cache,
+                          const int32_t* slots, int page_size, int write_kv, hipStream_t stream) {
+  qk_norm_rope_store_vec_kernel<T, W, MAXV, FP4><<<tokens, threads, shmem, stream>>>(
+      static_cast<T*>(qkv), row_stride, positions, cos_sin, static_cast<const W*>(qw),
+      static_cast<const W*>(kw), eps, heads, kv_heads, head_dim, rotary_dim, static_cast<T*>(cache),
+      slots, page_size, write_kv);
+}
 template <typename T, typename W, int MAXV>
 static void launch_vec(int threads, size_t shmem, void* qkv, int64_t row_stride, const int32_t* positions,
                        const float* cos_sin, const void* qw, const void* kw, float eps, int tokens,
                        int heads, int kv_heads, int head_dim, int rotary_dim, void* cache,
                        const int32_t* slots, int page_size, int write_kv, hipStream_t stream) {
-  qk_norm_rope_store_vec_kernel<T, W, MAXV><<<tokens, threads, shmem, stream>>>(
-      static_cast<T*>(qkv), row_stride, positions, cos_sin, static_cast<const W*>(qw),
-      static_cast<const W*>(kw), eps, heads, kv_heads, head_dim, rotary_dim, static_cast<T*>(cache),
-      slots, page_size, write_kv);
+  if (write_kv == WRITE_FP4)
+    launch_vec_to<T, W, MAXV, true>(threads, shmem, qkv, row_stride, positions, cos_sin, qw, kw, eps, tokens, heads, kv_heads,
+                                    head_dim, rotary_dim, cache, slots, page_size, write_kv, stream);
+  else
+    launch_vec_to<T, W, MAXV, false>(threads, shmem, qkv, row_stride, positions, cos_sin, qw, kw, eps, tokens, heads, kv_heads,
+                                     head_dim, rotary_dim, cache, slots, page_size, write_kv, stream);
 }
 
 template <typename T, typename W>
@@ -340,6 +401,7 @@ static int launch(void* qkv, int64_t row_stride, const int32_t* positions, const
     } else return SE_ERR_SHAPE;
 #undef SE_QK_VEC
   } else {
+    if (write_kv == WRITE_FP4) return SE_ERR_SHAPE;      // the caller writes those with se_fp4_store
     const size_t shmem = static_cast<size_t>(width + heads + kv_heads) * sizeof(float);
     qk_norm_rope_store_kernel<T, W><<<tokens, 256, shmem, stream>>>(
         static_cast<T*>(qkv), row_stride, positions, cos_sin, static_cast<const W*>(qw),
@@ -364,6 +426,8 @@ extern "C" int se_qk_norm_rope_store(void* qkv, int64_t row_stride, const int32_
   if (pairing != 0 && pairing != 1) return SE_ERR_SHAPE;
   if ((q_weight == nullptr) != (k_weight == nullptr)) return SE_ERR_SHAPE;
   if (write_kv && (!cache || !slots || page_size <= 0)) return SE_ERR_SHAPE;
+  if (write_kv < 0 || write_kv > WRITE_FP4) return SE_ERR_SHAPE;
+  if (write_kv == WRITE_FP4 && (head_dim % FP4_GROUP || page_size % 32)) return SE_ERR_SHAPE;
   if (static_cast<int64_t>(heads + 2 * kv_heads) * head_dim > 15360) return SE_ERR_SHAPE;  // row kept in LDS
   if (dtype == SE_F32) {
     if (q_weight && weight_dtype != SE_F32) return SE_ERR_SHAPE;

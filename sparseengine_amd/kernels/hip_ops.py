@@ -60,10 +60,12 @@ def _require(cond: bool, message: str):
 
 def _same_device(*tensors):
     """All on one device, and that the current one: a launch goes to the current device's current stream."""
-    device = tensors[0].device
-    _require(all(t is None or t.device == device for t in tensors), "the tensors of a call must be on one device")
-    _require(device.type != "cuda" or device.index == torch.cuda.current_device(),
-             "the tensors of a call must be on the current device")
+    device = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ValueError("the tensors of a call must be on one device")
+    if device >= 0 and device != torch.cuda.current_device():
+        raise ValueError("the tensors of a call must be on the current device")
 
 
 def _i32(t: torch.Tensor, name: str):
@@ -363,7 +365,11 @@ class HipKernels:
         tokens = qkv.shape[0]
         width = (heads + 2 * kv_heads) * head_dim
         int32 = torch.int32
-        if cache is not None and cache.dtype == torch.uint8:
+        fp4 = cache is not None and cache.dtype == torch.uint8
+        # what the short way below also takes of a cache in 4 bits: its kernel's form for rows of whole vectors
+        if fp4 and not (_SHORT_WAYS and head_dim % 32 == 0 and page_size % 32 == 0 and pairing == "neox" and rotary_dim % 16 == 0
+                        and qkv.stride(0) % 8 == 0 and q_weight is not None and k_weight is not None and cos_sin is not None
+                        and not ((qkv.data_ptr() | q_weight.data_ptr() | k_weight.data_ptr() | cache.data_ptr() | cos_sin.data_ptr()) & 15)):
             return self._store_fp4(qkv, positions, cos_sin, q_weight, k_weight, eps, heads, kv_heads, head_dim,
                                    rotary_dim, cache, slots, page_size, pairing, per_head_norm)
         # the call of every layer (norm weights, a rotation table, the cache write) in one expression; a call that
@@ -377,17 +383,29 @@ class HipKernels:
                 and q_weight.shape == (heads * head_dim,) and k_weight.shape == (kv_heads * head_dim,)
                 and q_weight.dtype == k_weight.dtype and q_weight.is_contiguous() and k_weight.is_contiguous()
                 and slots.dtype == int32 and slots.is_contiguous() and slots.numel() == tokens
-                and cache.dtype == qkv.dtype and cache.is_contiguous() and cache.dim() == 5
-                and tuple(cache.shape[1:]) == (2, kv_heads, page_size, head_dim)
+                and (fp4 or cache.dtype == qkv.dtype) and cache.is_contiguous() and cache.dim() == 5
+                and cache.shape[1:] == (2, kv_heads, page_size, head_dim * 17 // 32 if fp4 else head_dim)
                 and page_size % 8 == 0 and head_dim % 8 == 0):
+            if fp4:
+                _same_device(qkv, cache, slots)
             aligned = not ((qkv.data_ptr() | q_weight.data_ptr() | k_weight.data_ptr() | cache.data_ptr()
                             | cos_sin.data_ptr()) & 15)
             _check(_fn.get("rope_kv", "se_qk_norm_rope_store")(
                 _ptr(qkv), qkv.stride(0), _ptr(positions), _ptr(cos_sin), _ptr(q_weight), _ptr(k_weight), float(eps),
-                tokens, heads, kv_heads, head_dim, rotary_dim, _ptr(cache), _ptr(slots), page_size, 1,
+                tokens, heads, kv_heads, head_dim, rotary_dim, _ptr(cache), _ptr(slots), page_size, 2 if fp4 else 1,
                 _code(qkv.dtype), _code(q_weight.dtype), int(aligned), self.ROTARY_PAIRINGS[pairing], 0, _stream()),
                 "qk_norm_rope_store")
             return
+        if fp4:
+            return self._store_fp4(qkv, positions, cos_sin, q_weight, k_weight, eps, heads, kv_heads, head_dim,
+                                   rotary_dim, cache, slots, page_size, pairing, per_head_norm)
+        self._rope(qkv, positions, cos_sin, q_weight, k_weight, eps, heads, kv_heads, head_dim, rotary_dim, cache, slots,
+                   page_size, pairing, per_head_norm)
+
+    def _rope(self, qkv, positions, cos_sin, q_weight, k_weight, eps, heads, kv_heads, head_dim, rotary_dim, cache, slots,
+              page_size, pairing, per_head_norm):
+        tokens = qkv.shape[0]
+        width = (heads + 2 * kv_heads) * head_dim
         _require(qkv.dim() == 2 and qkv.shape[1] == width and qkv.stride(1) == 1, "qkv shape")
         _i32(positions, "positions")
         _require(positions.numel() == tokens, "positions length")
@@ -402,10 +420,11 @@ class HipKernels:
                      "qk norm weight shapes")
         if pairing not in self.ROTARY_PAIRINGS:
             raise ValueError(f"rotary pairing {pairing!r} is unknown ({', '.join(self.ROTARY_PAIRINGS)})")
-        write_kv = cache is not None
+        write_kv = 0 if cache is None else 2 if cache.dtype == torch.uint8 else 1
         if write_kv:
             _i32(slots, "slots")
             _require(slots.numel() == tokens, "slots length")
+        if write_kv == 1:
             _require(cache.dtype == qkv.dtype and cache.is_contiguous() and cache.dim() == 5
                      and tuple(cache.shape[1:]) == (2, kv_heads, page_size, head_dim), "cache layout")
             if page_size % 8 or head_dim % 8:
@@ -414,7 +433,7 @@ class HipKernels:
         _check(_fn.get("rope_kv", "se_qk_norm_rope_store")(
             _ptr(qkv), qkv.stride(0), _ptr(positions), _ptr(cos_sin) if rotary_dim else None,
             _ptr(q_weight), _ptr(k_weight), float(eps), tokens, heads, kv_heads, head_dim, rotary_dim,
-            _ptr(cache), _ptr(slots), page_size, int(write_kv), _code(qkv.dtype), wd,
+            _ptr(cache), _ptr(slots) if write_kv else None, page_size, write_kv, _code(qkv.dtype), wd,
             int(all(t is None or t.data_ptr() % 16 == 0 for t in (qkv, q_weight, k_weight, cache, cos_sin))),
             self.ROTARY_PAIRINGS[pairing], int(bool(per_head_norm and q_weight is not None)), _stream()),
             "qk_norm_rope_store")
@@ -433,20 +452,33 @@ class HipKernels:
             raise KernelShapeError("a 4-bit cache has to begin on a multiple of 16 bytes")
         return page
 
+    def _writes_fp4(self, qkv, cos_sin, q_weight, k_weight, rotary_dim, cache, pairing, per_head_norm) -> bool:
+        """Whether the norm and rotation kernel writes a 4-bit cache itself: in its form for rows of whole vectors, of
+        any number (6 us against 9 with a second kernel at 64 tokens of 48 + 8 + 8 heads of 128, 40 against 42 at 4096)."""
+        if pairing != "neox" or rotary_dim // 2 % 8:
+            return False
+        if q_weight is None and not rotary_dim or per_head_norm and q_weight is not None:
+            return False
+        return all(t is None or t.data_ptr() % 16 == 0 for t in (qkv, q_weight, k_weight, cache, cos_sin if rotary_dim else None))
+
     def _store_fp4(self, qkv, positions, cos_sin, q_weight, k_weight, eps, heads, kv_heads, head_dim, rotary_dim, cache,
                    slots, page_size, pairing, per_head_norm):
         tokens = qkv.shape[0]
         self._fp4_cache(cache, head_dim, page_size)
         _require(cache.shape[2] == kv_heads, "4-bit cache layout")
-        _i32(slots, "slots")
-        _require(slots.numel() == tokens, "slots length")
-        _require(qkv.dim() == 2 and qkv.shape[1] == (heads + 2 * kv_heads) * head_dim and qkv.stride(1) == 1, "qkv shape")
         _same_device(qkv, cache, slots)
+        fused = self._writes_fp4(qkv, cos_sin, q_weight, k_weight, rotary_dim, cache, pairing, per_head_norm)
+        if not fused:
+            _i32(slots, "slots")
+            _require(slots.numel() == tokens, "slots length")
+            _require(qkv.dim() == 2 and qkv.shape[1] == (heads + 2 * kv_heads) * head_dim and qkv.stride(1) == 1, "qkv shape")
         if qkv.stride(0) % 8 or qkv.data_ptr() % 16:
             raise KernelShapeError("4-bit cache write: qkv rows have to begin on multiples of 16 bytes")
-        if q_weight is not None or rotary_dim:
-            self.qk_norm_rope_store(qkv, positions, cos_sin, q_weight, k_weight, eps, heads, kv_heads, head_dim,
-                                    rotary_dim, None, None, page_size, pairing=pairing, per_head_norm=per_head_norm)
+        if fused or q_weight is not None or rotary_dim:
+            self._rope(qkv, positions, cos_sin, q_weight, k_weight, eps, heads, kv_heads, head_dim, rotary_dim,
+                       cache if fused else None, slots, page_size, pairing, per_head_norm)
+        if fused:
+            return
         _check(_fn.get("cache_fp4", "se_fp4_store")(
             _ptr(qkv), qkv.stride(0), _ptr(slots), tokens, heads, kv_heads, head_dim, _ptr(cache), page_size,
             _code(qkv.dtype), _stream()), "qk_norm_rope_store (4-bit cache)")
@@ -492,7 +524,7 @@ class HipKernels:
                 kv_heads, page, head_dim, _code(q.dtype), _stream()), "paged_attention (unpacking 4-bit pages)")
         if not direct:
             if q.dtype == torch.bfloat16 and head_dim <= 256:
-                self._run_attention_work(q, scratch, scratch_table, work, out, scale, window, lse)
+                self._run_attention_work(q, scratch, scratch_table, work, out, scale, window, lse, unpacked=True)
             else:
                 self._paged_attention_generic(q, scratch, scratch_table, meta, out, scale, window, lse)
             return
@@ -627,6 +659,20 @@ class HipKernels:
         kv_heads, page_size = cache.shape[2], cache.shape[3]
         _require(q.stride(2) == 1 and q.stride(1) == head_dim, "q heads must be dense")
         fp4 = cache.dtype == torch.uint8
+        if fp4 and _SHORT_WAYS and getattr(meta, "work", None) and getattr(meta, "item_q_len", None) is not None:
+            # a step of few rows per item with its work list prepared, in one expression; every other call, and one that
+            # fails a check, takes the long way, which names what is wrong
+            work, table = meta.work.get((heads // kv_heads if kv_heads else 0, window, "fp4")), meta.block_table
+            if (work is not None and not work.num_block_units and heads % kv_heads == 0 and scale > 0
+                    and q.dtype == torch.bfloat16 and head_dim in FP4_HEAD_DIMS and q.stride(0) % 8 == 0
+                    and cache.dim() == 5 and cache.shape[1] == 2 and cache.shape[4] * 32 == head_dim * 17 and page_size % 32 == 0
+                    and cache.is_contiguous()
+                    and (lse is None or lse.dtype == torch.float32 and lse.is_contiguous() and lse.shape == (tokens, heads))
+                    and out.shape == (tokens, heads * head_dim) and out.stride(1) == 1 and out.dtype == torch.bfloat16
+                    and out.stride(0) % 8 == 0 and table.dtype == torch.int32 and table.dim() == 2 and table.stride(1) == 1
+                    and meta.token_row.numel() == tokens and not (q.data_ptr() | cache.data_ptr() | out.data_ptr()) & 15):
+                _same_device(q, cache, out, lse, table)
+                return self._run_attention_work(q, None, None, work, out, scale, window, lse, fp4=(cache, table))
         _require(fp4 or (cache.dim() == 5 and cache.shape[1] == 2 and cache.shape[4] == head_dim
                          and cache.is_contiguous() and cache.dtype == q.dtype), "cache layout")
         if lse is not None:
@@ -683,15 +729,16 @@ class HipKernels:
                 meta.work[key] = work
         return work
 
-    def _run_attention_work(self, q, cache, block_table, work, out, scale, window, lse, fp4=None):
+    def _run_attention_work(self, q, cache, block_table, work, out, scale, window, lse, fp4=None, unpacked=False):
         """Matrix-core path: work units (row tile x key range) from the step's item lengths.  ``fp4``: None, or
-        (4-bit cache, its block table) that the single-wavefront units read; ``cache`` is then what the blocks read."""
+        (4-bit cache, its block table) that the single-wavefront units read; ``cache`` is then what the blocks read.
+        ``unpacked``: ``cache`` is the call's own copy of 4-bit pages."""
         tokens, heads, head_dim = q.shape
         kv_heads, page_size = (cache if fp4 is None else fp4[0]).shape[2:4]
         part_o = part_ml = None
         if work.num_slots:                    # key ranges leave partial results for the merge
             need = work.num_slots * kv_heads * 16
-            if fp4 is not None:               # the call's own: nothing of another stream's or graph's is reused
+            if fp4 is not None or unpacked:   # the call's own, as its unpacked pages: nothing of another stream's or graph's is reused
                 part_o = torch.empty(need * head_dim, dtype=torch.float32, device=q.device)
                 part_ml = torch.empty(need * 2, dtype=torch.float32, device=q.device)
             else:

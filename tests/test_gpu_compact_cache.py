@@ -12,6 +12,7 @@ import pytest
 import torch
 
 from sparseengine_amd.cache import layout
+from sparseengine_amd.kernels import hip_ops
 from sparseengine_amd.kernels.hip_ops import KernelShapeError
 from tests import backends
 from tests import compact_oracle as oracle
@@ -145,6 +146,35 @@ def test_store_holds_what_qkv_holds(hip, dtype, tokens, heads, kv, d, page, rota
             for h in range(kv):
                 assert oracle.token_of(after, slot // page, which, h, slot % page, d) == held[i, h].tolist()
     assert torch.equal(after, expected)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,heads,kv,d,page,rotary,norm", [(3, 48, 8, 128, 64, 64, "flat"), (40, 3, 1, 64, 32, 64, None),
+                                                                (130, 6, 3, 96, 32, 16, "flat"), (600, 2, 1, 32, 64, 32, None)])
+def test_store_in_one_kernel_and_in_two(hip, monkeypatch, dtype, tokens, heads, kv, d, page, rotary, norm):
+    """The rotation's kernel that writes 4 bits itself leaves the bytes that a kernel of its own reads back and writes,
+    also for elements that are not finite."""
+    emulator_skips(tokens * (heads + 2 * kv) * d, 1e6)
+    rng = np.random.default_rng(tokens)
+    qkv = randn(tokens, (heads + 2 * kv) * d, dtype=dtype, seed=1)
+    qkv[:, heads * d:] *= torch.exp(2 * torch.randn(2 * kv * d, generator=torch.Generator().manual_seed(3)))[None].to(dtype)
+    qkv[0, -1], qkv[1, -d], qkv[tokens - 1, heads * d + 1] = float("nan"), float("inf"), -float("inf")
+    angle = torch.rand(tokens, rotary // 2, generator=torch.Generator().manual_seed(2)) * 6
+    table = torch.cat([angle.cos(), angle.sin()], -1).to(DEV)
+    w = [None, None] if norm is None else [(1 + 0.1 * randn(n * d, dtype=torch.float32, seed=4)).to(dtype).to(DEV) for n in (heads, kv)]
+    pages = -(-tokens // page) + 1
+    slots = torch.tensor(rng.permutation(pages * page)[:tokens], dtype=torch.int32)
+    slots[2] = -1
+    slots, positions = slots.to(DEV), torch.arange(tokens, dtype=torch.int32).to(DEV)
+    ways = []
+    for ours in (hip, type("TwoKernels", (type(hip),), dict(_writes_fp4=lambda self, *a: False))()):
+        rows, cache = qkv.clone().to(DEV), torch.full((pages, 2, kv, page, layout.fp4_row_bytes(d)), 77, dtype=torch.uint8).to(DEV)
+        if ours is not hip:
+            monkeypatch.setattr(hip_ops, "_SHORT_WAYS", False)
+        ours.qk_norm_rope_store(rows, positions, table, *w, 1e-5, heads, kv, d, rotary, cache, slots, page)
+        ways.append((rows.cpu().view(torch.uint8), cache.cpu()))
+    assert torch.equal(ways[0][0], ways[1][0]) and torch.equal(ways[0][1], ways[1][1])
+    assert (ways[0][1] == 255).any()
 
 
 def test_store_borders(hip):
@@ -462,6 +492,81 @@ def test_a_request_in_4_bits_from_store_to_eviction(hip, dtype):
     out1, lse1 = torch.empty(1, heads * d, dtype=dtype).to(DEV), torch.empty(1, heads).to(DEV)
     hip.paged_attention(q[-1:], cache, after, out1, d ** -0.5, lse=lse1)
     check_attention(out1, lse1, q.cpu()[-1:], lambda w: lambda i: left[w], [keep], [1], d ** -0.5, 0, dtype)
+
+
+@pytest.mark.skipif(backends.ACTIVE.name != "hip", reason="graphs and streams are the GPU's")
+@pytest.mark.parametrize("graphs", [1, 2])
+def test_a_captured_step_on_another_stream(hip, graphs):
+    """Store, attention, weights and eviction recorded into graphs on a stream of their own, replayed in turn on new
+    numbers: each replay gives what eager calls give, whichever ran between."""
+    heads, kv, d, page, ctx, keep, bf16 = 12, 2, 64, 32, [200, 37, 700], 30, torch.bfloat16
+    scale, items, span = d ** -0.5, len(ctx), 96       # a portion of 96 tokens beside single ones: the unpacked way too
+
+    class Step:
+        def __init__(self, seed):
+            new = [1, 1, span] if seed % 2 else [1, 1, 1]
+            rng = np.random.default_rng(seed)
+            self.meta, self.pages = oracle.step(ctx, new, page, DEV, rng)
+            fresh = -(-keep // page)
+            total = self.pages + fresh * items
+            self.cache, _ = make_layer("fp4", total, kv, page, d, seed, bf16)
+            self.cache = self.cache.to(DEV)
+            self.qkv = torch.zeros(sum(new), (heads + 2 * kv) * d, dtype=bf16).to(DEV)
+            table = self.meta.block_table.cpu()
+            slots = [table[i, p // page] * page + p % page for i in range(items) for p in range(ctx[i] - new[i], ctx[i])]
+            self.slots = torch.tensor([int(x) for x in slots], dtype=torch.int32).to(DEV)
+            angle = torch.rand(max(ctx), d // 4) * 6
+            self.angles = torch.cat([angle.cos(), angle.sin()], -1).to(DEV)
+            self.out, self.lse = torch.zeros(sum(new), heads * d, dtype=bf16).to(DEV), torch.zeros(sum(new), heads).to(DEV)
+            self.weights = torch.zeros(total, kv, page).to(DEV)
+            self.lengths = torch.tensor(ctx, dtype=torch.int32).to(DEV)
+            self.new_table = torch.arange(self.pages, total, dtype=torch.int32).reshape(items, fresh).to(DEV)
+            self.kept = torch.zeros(items, kv, keep, dtype=torch.int32).to(DEV)
+
+        def run(self):
+            hip.qk_norm_rope_store(self.qkv, self.meta.positions, self.angles, None, None, 1e-6, heads, kv, d, d // 2, self.cache, self.slots, page)
+            hip.paged_attention(self.qkv[:, :heads * d].view(-1, heads, d), self.cache, self.meta, self.out, scale, lse=self.lse)
+            hip.attention_weights(self.qkv[:, :heads * d].view(-1, heads, d), self.cache, self.meta, self.lse, self.weights, scale)
+            hip.evict_tokens(self.cache, self.weights, self.meta.block_table, self.lengths, self.new_table, keep, 4, self.kept, longest=max(ctx))
+
+        def results(self):
+            return [t.clone().cpu() for t in (self.qkv, self.out, self.lse, self.weights, self.kept, self.cache)]
+
+    steps = [Step(seed) for seed in range(1, 1 + graphs)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    recorded = []
+    with torch.cuda.stream(stream):
+        for s in steps:
+            s.run()
+    stream.synchronize()
+    for s in steps:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            s.run()
+        recorded.append(graph)
+    for turn in range(3):
+        given = [randn(*s.qkv.shape, dtype=bf16, seed=10 * turn + i) for i, s in enumerate(steps)]
+        wanted = []
+        for s, x in zip(steps, given):      # eager, on the default stream
+            start = s.cache.clone()
+            s.qkv.copy_(x)
+            s.weights.zero_()
+            s.run()
+            wanted.append(s.results())
+            s.cache.copy_(start)
+        torch.cuda.synchronize()
+        for s, x in zip(steps, given):
+            s.qkv.copy_(x)
+            s.weights.zero_()
+            s.kept.zero_()
+        torch.cuda.synchronize()
+        for graph in recorded:
+            graph.replay()
+        torch.cuda.synchronize()
+        for s, want in zip(steps, wanted):
+            for got, expected in zip(s.results(), want):
+                assert torch.equal(got.flatten().view(torch.uint8), expected.flatten().view(torch.uint8)), turn
 
 
 # ---------------------------------------------------------------------------------------------- refusals
