@@ -23,6 +23,11 @@ __device__ __forceinline__ uint32_t order_word(float w) {     // larger weights,
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
+// the word of a token's weight; a token whose page is gone comes behind every weight
+__device__ __forceinline__ uint32_t word_of(int page, float w) {
+  return page < 0 ? 1u : order_word(w);
+}
+
 #define CHOOSE_WAVES (CHOOSE_THREADS / SE_WAVE)
 #define CHOOSE_COPIES 16
 
@@ -78,7 +83,7 @@ choose_tokens_kernel(const float* __restrict__ weights, const int32_t* __restric
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const bool candidate = base + r * CHOOSE_THREADS + tid < candidates;
-      id[r] = table[candidate ? page : 0];
+      id[r] = candidate ? table[page] : 0;
       at[r] = candidate ? off : 0;
       page += step_pages;
       off += step_off;
@@ -89,8 +94,8 @@ choose_tokens_kernel(const float* __restrict__ weights, const int32_t* __restric
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const float w = weights[(static_cast<int64_t>(id[r]) * kv_heads + kvh) * page_size + at[r]];
-      word[r] = base + r * CHOOSE_THREADS + tid < candidates ? order_word(w) : 0u;
+      const float w = weights[(static_cast<int64_t>(max(id[r], 0)) * kv_heads + kvh) * page_size + at[r]];
+      word[r] = base + r * CHOOSE_THREADS + tid < candidates ? word_of(id[r], w) : 0u;
     }
   };
   uint32_t word[R];
@@ -110,7 +115,8 @@ choose_tokens_kernel(const float* __restrict__ weights, const int32_t* __restric
     for (int r = 0; r < R; ++r) count(word[r]);
     int page = (R * CHOOSE_THREADS + tid) / page_size, off = (R * CHOOSE_THREADS + tid) - page * page_size;
     for (int i = R * CHOOSE_THREADS + tid; i < candidates; i += CHOOSE_THREADS) {
-      count(order_word(weights[(static_cast<int64_t>(table[page]) * kv_heads + kvh) * page_size + off]));
+      const int id = table[page];
+      count(word_of(id, weights[(static_cast<int64_t>(max(id, 0)) * kv_heads + kvh) * page_size + off]));
       page += step_pages;
       off += step_off;
       if (off >= page_size) {

@@ -136,6 +136,8 @@ class ModelRunner:
             return cap
         free, total = torch.cuda.mem_get_info(self.device)
         usable = free - int((1.0 - utilization) * total) - (2 << 30)      # 2 GiB kept for step buffers
+        if self.kv_dtype != self.dtype:      # and what a step's portions of two longest prompts unpack for a layer
+            usable -= 2 * self.max_model_len * max(bytes_per_token(r, self.dtype) for r in requests.values() if isinstance(r, PagedKVRequest))
         if usable <= per_token * max([self.kv_page_size] + [r.page_size or 0 for r in requests.values()
                                                             if isinstance(r, PagedKVRequest)]):
             raise RuntimeError("no GPU memory is left for the cache after the weights")

@@ -75,6 +75,14 @@ FP4_WAVES = 1024            # ranges wanted at head sizes from 128 on, while the
 FP4_MANY_WAVES = 2048       # else
 FP4_MIN_SPLIT_KEYS = 128
 FP4_WHOLE_KEYS = 160        # a step none of whose contexts is longer is not split at all
+# Items in blocks read unpacked pages, which takes a launch and writes and reads four times the bytes, but then every
+# product costs less than half: 5.6 against about 2.5 us a row tile and 32768 keys (48:8 heads of 128, one request).  16,
+# 64, 128 and 192 rows at 4096 keys take 48, 55, 59 and 63 us in blocks, 18, 32, 52 and 69 directly; 16, 32 and 128 at
+# 32768 keys 74, 82 and 175 against 47, 87 and 282; 32:8 heads of 64: 128 and 256 rows at 4096 keys 41 and 47 against 29
+# and 48, 32 and 96 at 32768 keys 53 and 70 against 38 and 88.  An item with at least so many tiles goes in blocks if
+# the step's items together have so many tiles beyond that, times the keys they read.
+FP4_BLOCK_TILES = 8
+FP4_BLOCK_WORK = 196608
 
 _native = None      # the compiled builder (csrc/host_work.hip)
 
@@ -100,14 +108,14 @@ _BAD_LENGTHS = "attention work: every item needs at least one new token and no m
 
 def build_attention_work(q_len, ctx_len, group: int, kv_heads: int, window: int = 0,
                          target_waves: int = TARGET_WAVES, head_dim: int = 0,
-                         min_split_keys: int = MIN_SPLIT_KEYS) -> AttentionWork:
+                         min_split_keys: int = MIN_SPLIT_KEYS, block_tiles: int = TILES_PER_BLOCK // 2) -> AttentionWork:
     """The work lists of one step, from the compiled builder; ``build_attention_work_numpy`` states
     the rules and gives the same lists (the tests compare the two), about twenty times slower."""
     lib = _native_library()
     q = np.ascontiguousarray(q_len, dtype=np.int64)
     c = np.ascontiguousarray(ctx_len, dtype=np.int64)
     rules = np.asarray([target_waves, min_split_keys, MAX_SPLITS, TILES_PER_BLOCK, TILED_MAX_HEAD_DIM,
-                        TARGET_BLOCKS, MIN_BLOCK_KEYS, PREFIX_PER_PORTION], dtype=np.int64)
+                        TARGET_BLOCKS, MIN_BLOCK_KEYS, PREFIX_PER_PORTION, block_tiles], dtype=np.int64)
     plan = np.empty((q.size, 6), dtype=np.int64)
     counts = np.empty(4, dtype=np.int64)
     i64p, i32p = ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int32)
@@ -130,11 +138,23 @@ def build_fp4_attention_work(q_len, ctx_len, group: int, kv_heads: int, window: 
     """The work lists of a step over a cache in 4 bits: ranges that together are no more than fill the chip once (an
     item's last range is a partial one, so one is taken off the number wanted for each tile)."""
     q = np.asarray(q_len, dtype=np.int64)
-    tiles = int(((q * group + 15) // 16)[~items_in_blocks(q, group, head_dim)].sum()) * kv_heads
+    block_tiles = fp4_block_tiles(q, ctx_len, group, window)
+    tiles = int(((q * group + 15) // 16)[~items_in_blocks(q, group, head_dim, block_tiles)].sum()) * kv_heads
     wanted = FP4_WAVES if head_dim >= 128 and 4 * tiles <= FP4_WAVES else FP4_MANY_WAVES
     if q.size and int(np.max(ctx_len)) <= FP4_WHOLE_KEYS:
         wanted = 0
-    return build_attention_work(q_len, ctx_len, group, kv_heads, window, max(1, wanted - tiles), head_dim, FP4_MIN_SPLIT_KEYS)
+    return build_attention_work(q_len, ctx_len, group, kv_heads, window, max(1, wanted - tiles), head_dim, FP4_MIN_SPLIT_KEYS,
+                                block_tiles)
+
+
+def fp4_block_tiles(q_len, ctx_len, group: int, window: int) -> int:
+    """The tiles an item needs to go in blocks in a step over a cache in 4 bits."""
+    q, c = np.asarray(q_len, dtype=np.int64), np.asarray(ctx_len, dtype=np.int64)
+    beyond = np.maximum((q * group + 15) // 16 - FP4_BLOCK_TILES, 0)
+    if not beyond.any():
+        return FP4_BLOCK_TILES + 1
+    reach = np.minimum(c, window + q) if window else c
+    return FP4_BLOCK_TILES if int((beyond * reach).sum()) >= FP4_BLOCK_WORK else 1 << 30
 
 
 FP4_HEAD_DIMS = (64, 128, 256)      # head sizes that the 4-bit attention kernel is built for
@@ -144,7 +164,8 @@ def fp4_unpack_list(q_len, ctx_len, group: int, head_dim: int, page: int, window
     """Which pages of a 4-bit cache a step reads through unpacked copies (those of the block kernel's items, or of all):
     int32 ``[n, 2]`` (item, column of the block table), and int32 ``[items, columns]`` where each lies among them."""
     q_len, ctx_len = np.asarray(q_len, dtype=np.int64), np.asarray(ctx_len, dtype=np.int64)
-    chosen = items_in_blocks(q_len, group, head_dim) if only_blocks else np.ones(q_len.size, dtype=bool)
+    chosen = (items_in_blocks(q_len, group, head_dim, fp4_block_tiles(q_len, ctx_len, group, window)) if only_blocks
+              else np.ones(q_len.size, dtype=bool))
     low = np.maximum(0, ctx_len - q_len - window + 1) if window else np.zeros_like(ctx_len)
     first, until = low // page, -(-ctx_len // page)
     column = np.arange(int(until.max()))[None, :]
@@ -155,17 +176,17 @@ def fp4_unpack_list(q_len, ctx_len, group: int, head_dim: int, page: int, window
     return pairs, table
 
 
-def items_in_blocks(q_len, group: int, head_dim: int) -> np.ndarray:
-    """Which items go to the block kernel: those with at least half a block of tiles."""
+def items_in_blocks(q_len, group: int, head_dim: int, block_tiles: int = TILES_PER_BLOCK // 2) -> np.ndarray:
+    """Which items go to the block kernel: those with at least half a block of tiles, or ``block_tiles``."""
     tiles = (np.asarray(q_len, dtype=np.int64) * group + 15) // 16
     if not head_dim or head_dim % 32 or head_dim > TILED_MAX_HEAD_DIM:
         return np.zeros(tiles.size, dtype=bool)
-    return tiles >= TILES_PER_BLOCK // 2
+    return tiles >= block_tiles
 
 
 def build_attention_work_numpy(q_len, ctx_len, group: int, kv_heads: int, window: int = 0,
                                target_waves: int = TARGET_WAVES, head_dim: int = 0,
-                               min_split_keys: int = MIN_SPLIT_KEYS) -> AttentionWork:
+                               min_split_keys: int = MIN_SPLIT_KEYS, block_tiles: int = TILES_PER_BLOCK // 2) -> AttentionWork:
     """``head_dim``: 0 keeps every item on the one-wavefront kernel (callers that do not know it).
 
     Items with at least half a block of tiles (prompt portions) go to the block kernel, the others
@@ -179,7 +200,7 @@ def build_attention_work_numpy(q_len, ctx_len, group: int, kv_heads: int, window
     q_start = np.concatenate(([0], np.cumsum(q_len)[:-1]))      # items' tokens lie one after the other
     tiles = (q_len * group + 15) // 16
     reach = np.minimum(ctx_len, window + q_len) if window else ctx_len      # keys an item's tiles can read
-    in_blocks = items_in_blocks(q_len, group, head_dim)
+    in_blocks = items_in_blocks(q_len, group, head_dim, block_tiles)
 
     def keys_per_unit(units_per_item, wanted: int, least: int) -> int:
         """Keys of a range so that all ranges together number about ``wanted``."""

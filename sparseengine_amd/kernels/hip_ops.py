@@ -499,14 +499,13 @@ class HipKernels:
 
     def _paged_attention_fp4(self, q, cache, meta, out, scale, window, lse):
         """Attention over a 4-bit cache.  In bfloat16, at the head sizes its kernel takes, items of few rows (the
-        work list's units) are read in 4 bits; the pages of items of many rows (its blocks: a page is then read
-        once per block of rows, and turning it into bfloat16 each time would cost more than the products), and of
-        everything else, are unpacked to a temporary cache in the engine's own layout first."""
+        work list's units) are read in 4 bits; the pages of items of many rows over long contexts (its blocks,
+        ``fp4_block_tiles``: a page is then read once per block of rows, and turning it into bfloat16 each time
+        would cost more than the products), and of everything else, are unpacked to a temporary cache in the engine's own layout first."""
         tokens, heads, head_dim = q.shape
         page = self._fp4_cache(cache, head_dim)
         kv_heads = cache.shape[2]
-        if getattr(meta, "item_q_len", None) is None:
-            raise ValueError("attention over a 4-bit cache needs the step's items (item_q_len, item_ctx_len)")
+        self._check_items(meta, tokens, page, "attention over a 4-bit cache")
         _require(scale > 0, "attention over a 4-bit cache: scale must be positive")
         direct = q.dtype == torch.bfloat16 and head_dim in FP4_HEAD_DIMS
         group = heads // kv_heads
@@ -568,9 +567,9 @@ class HipKernels:
         _code(q.dtype)
         if heads % kv_heads:
             raise KernelShapeError(f"attention weights: {heads} heads do not divide into {kv_heads} kv heads")
-        if page % 8 or head_dim % 8 or head_dim > 512 or q.stride(0) % 8 or q.data_ptr() % 16:
+        if page % 8 or head_dim % 8 or head_dim > 512 or q.stride(0) % 8 or (q.data_ptr() | cache.data_ptr()) % 16:
             raise KernelShapeError(f"attention weights: page_size {page} and head_dim {head_dim} in steps of 8 (head_dim "
-                                   "at most 512), q rows on multiples of 16 bytes")
+                                   "at most 512), q rows and the cache on multiples of 16 bytes")
         for name, w in (("out", out), ("previous", previous)):
             _require(w is None or (w.dtype == torch.float32 and w.is_contiguous() and tuple(w.shape) == (pages, kv_heads, page)),
                      f"attention weights: {name} must be contiguous float32 [pages, kv_heads, page_size]")
@@ -591,16 +590,22 @@ class HipKernels:
             meta.block_table.stride(0), _ptr(item_meta), items, longest, most_new, _ptr(lse), _ptr(previous), _ptr(out), heads, kv_heads,
             head_dim, page, float(scale), int(window or 0), _code(q.dtype), _ptr(workspace), _stream()), "attention_weights")
 
-    def _items(self, meta, tokens: int, page: int):
-        """(number of items, longest context, most new tokens, int32 ``[3, items]`` on the device) of a step, checked."""
+    @staticmethod
+    def _check_items(meta, tokens: int, page: int, what: str):
+        """The items' new tokens and contexts (numpy), and the longest context."""
         if getattr(meta, "item_q_len", None) is None:
-            raise ValueError("attention weights need the step's items (item_q_len, item_ctx_len)")
+            raise ValueError(f"{what} needs the step's items (item_q_len, item_ctx_len)")
         q_len, ctx_len = np.asarray(meta.item_q_len), np.asarray(meta.item_ctx_len)
         _require(q_len.size == ctx_len.size and q_len.size <= meta.block_table.shape[0] and bool((q_len >= 1).all())
                  and bool((q_len <= ctx_len).all()) and int(q_len.sum()) == tokens,
                  "items: every item needs at least one new token and no more than its context, together the step's tokens")
-        longest = int(ctx_len.max())
+        longest = int(ctx_len.max()) if q_len.size else 0
         _require(longest <= meta.block_table.shape[1] * page, "the block table has too few columns for the longest item")
+        return q_len, ctx_len, longest
+
+    def _items(self, meta, tokens: int, page: int):
+        """(number of items, longest context, most new tokens, int32 ``[3, items]`` on the device) of a step, checked."""
+        q_len, ctx_len, longest = self._check_items(meta, tokens, page, "attention weights")
         item_meta = getattr(meta, "item_meta", None)
         if item_meta is None:
             start = np.concatenate(([0], np.cumsum(q_len)[:-1]))
@@ -616,7 +621,8 @@ class HipKernels:
         ceil(keep / page_size)]``), with their weights.  ``kept`` (int32 ``[items, kv_heads, keep]``) receives their
         old places, ascending, -1 behind the last where a request has fewer.  ``cache`` is a layer in float32,
         bfloat16 or 4 bits.  The new pages must be none of the requests' old ones and no two the same; the old
-        pages stay as they are.  Rows of ``new_table`` with entries below 0 are filled up to those."""
+        pages stay as they are.  Old tokens whose page is below 0 (given back) go first, and a new place of one that
+        stays all the same is left as it was, as are the places of new pages below 0."""
         fp4 = cache.dtype == torch.uint8
         _require(cache.dim() == 5 and cache.shape[1] == 2 and cache.is_contiguous() and cache.dtype in self._CACHE_KINDS,
                  "cache layout")
@@ -693,6 +699,8 @@ class HipKernels:
             _same_device(q, cache, out, lse, meta.block_table)
             if q.stride(0) % 8 or out.stride(0) % 8 or q.data_ptr() % 16 or out.data_ptr() % 16:
                 raise KernelShapeError("attention over a 4-bit cache: rows of q and out have to begin on multiples of 16 bytes")
+            if tokens == 0:
+                return
             return self._paged_attention_fp4(q, cache, meta, out, float(scale), window, lse)
         if (q.dtype == torch.bfloat16 and head_dim % 32 == 0 and head_dim <= 256
                 and getattr(meta, "item_q_len", None) is not None):      # the step's items are known

@@ -56,6 +56,32 @@ def test_attention_and_weights(guard, case):
             C.test_weights_of_the_cached_keys(hip, BF16, "fp4", *C.ATTEND[case])
 
 
+def test_portions_in_unpacked_blocks(guard, monkeypatch):
+    with Emulated(guard=guard) as hip:
+        for case in C.ATTEND[11:14]:
+            C.test_attention_of_many_rows_in_unpacked_blocks(hip, monkeypatch, *case)
+        C.test_a_step_without_tokens(hip)
+        for kind in ("fp4", "own"):
+            C.test_eviction_from_a_table_with_pages_given_back(hip, kind)
+
+
+def test_which_portions_go_in_blocks():
+    """The builders agree, and the rule: at least 8 tiles, and enough work in the step."""
+    from sparseengine_amd.kernels import attention_work as aw
+    for q, ctx, window in (([1, 40, 300], [70, 9000, 700], 0), ([64], [64], 0), ([900, 2, 30], [4000, 9, 4096], 500)):
+        for block_tiles in (1, 4, 9, 1 << 30):
+            a = aw.build_attention_work(q, ctx, 6, 8, window, 900, 128, 64, block_tiles)
+            b = aw.build_attention_work_numpy(q, ctx, 6, 8, window, 900, 128, 64, block_tiles)
+            assert all((getattr(a, f) == getattr(b, f)).all() for f in ("units", "tasks", "block_units")) and a.num_slots == b.num_slots
+    blocks = lambda q, c, window=0, group=6: sorted(set(aw.build_fp4_attention_work(q, c, group, 8, window, 128).block_units[:, 0].tolist()))
+    assert blocks([1, 1], [9, 100000]) == [] and blocks([128], [4096]) == [] and blocks([192], [4096]) == [0]
+    assert blocks([16], [131072]) == [] and blocks([64], [32768]) == [0]
+    assert blocks([512, 16, 1], [16384, 16384, 70]) == [0] and blocks([512, 32], [16384, 16384]) == [0, 1]
+    assert blocks([192], [4096], window=100) == [] and blocks([512], [512]) == []
+    pairs, table = aw.fp4_unpack_list([512, 16, 22], [16384, 100, 40000], 6, 128, 64, 0, True)
+    assert set(pairs[:, 0].tolist()) == {0, 2} and len(pairs) == 256 + 625 and table[2, 624] == 880 and not table[1].any()
+
+
 def test_eviction_and_the_operators_together(guard):
     with Emulated(guard=guard, schedule="shuffled") as hip:
         for dtype in (F32, BF16):

@@ -18,11 +18,11 @@ emulated = pytest.mark.skipif(not backends.EmulatedBackend().available(), reason
 
 @emulated
 @pytest.mark.parametrize("key,dtype,guard,lengths,new,kwargs", [
-    ("C_loud", "bfloat16", "after", (33, 1), 3, {}), ("C_loud", "float32", "before", (34, 3), 2, {}),
+    ("C_loud", "bfloat16", "after", (33, 1), 3, {}), ("C_loud", "bfloat16", "before", (50, 1), 2, dict(blocks=True)), ("C_loud", "float32", "before", (34, 3), 2, {}),
     ("B_loud", "bfloat16", "before", (9, 35), 2, dict(max_num_batched_tokens=24))])
-def test_cache_in_4_bits(tmp_path, key, dtype, guard, lengths, new, kwargs):
+def test_cache_in_4_bits(tmp_path, monkeypatch, key, dtype, guard, lengths, new, kwargs):
     with backends.use(backends.EmulatedBackend(guard=guard)):
-        E.check_cache_in_4_bits(tmp_path, key, dtype, lengths, new, **kwargs)
+        E.check_cache_in_4_bits(tmp_path, monkeypatch, key, dtype, lengths, new, **kwargs)
 
 
 @emulated

@@ -7,6 +7,8 @@ result once: |error| <= 2^-8 sum p |v| + 2^-8 |o|, beside what float32 does to s
 error in float32: a score is a sum of D products, off by at most (D + 8) 2^-24 sum |q| |k| scale, and a relative error
 of that size goes into its exponential; the sums over n keys add n 2^-24; exponential and logarithm a few 2^-24 of
 their arguments."""
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 import torch
@@ -287,6 +289,41 @@ def test_attention_in_4_bits(hip, dtype, heads, kv, d, page, ctx, new, window):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("heads,kv,d,page,ctx,new,window", ATTEND[11:])
+def test_attention_of_many_rows_in_unpacked_blocks(hip, monkeypatch, heads, kv, d, page, ctx, new, window):
+    """Portions that the step's size alone would leave to the 4-bit kernel."""
+    from sparseengine_amd.kernels import attention_work
+    monkeypatch.setattr(attention_work, "FP4_BLOCK_WORK", 0)
+    test_attention_in_4_bits(hip, torch.bfloat16, heads, kv, d, page, ctx, new, window)
+    assert attention_work.build_fp4_attention_work(new, ctx, heads // kv, kv, window, d).block_units.size
+
+
+@pytest.mark.parametrize("new,ctx", [([1, 170], [300, 4200]), ([700], [700]), ([200, 3, 40], [1200, 40, 5000])])
+def test_portions_around_the_choice_of_a_kernel(hip, new, ctx):
+    heads, kv, d, page = 12, 2, 64, 64
+    emulator_skips(sum(c * n for c, n in zip(ctx, new)) * heads * d)
+    meta, cache, q, of = attention_case("fp4", torch.bfloat16, heads, kv, d, page, ctx, new, 0)
+    out, lse = torch.empty(sum(new), heads * d, dtype=torch.bfloat16).to(DEV), torch.empty(sum(new), heads).to(DEV)
+    hip.paged_attention(q.to(DEV), cache.to(DEV), meta, out, d ** -0.5, lse=lse)
+    check_attention(out, lse, q, of, ctx, new, d ** -0.5, 0, torch.bfloat16)
+
+
+def test_a_step_without_tokens(hip):
+    heads, kv, d, page, bf16 = 4, 2, 64, 32, torch.bfloat16
+    cache = torch.zeros(2, 2, kv, page, layout.fp4_row_bytes(d), dtype=torch.uint8).to(DEV)
+    i32 = lambda *shape: torch.zeros(*shape, dtype=torch.int32).to(DEV)
+    meta = SimpleNamespace(block_table=i32(0, 1), token_row=i32(0), positions=i32(0), page_size=page, item_q_len=np.zeros(0, dtype=np.int32),
+                           item_ctx_len=np.zeros(0, dtype=np.int32), item_meta=i32(3, 0), work={})
+    qkv = torch.zeros(0, (heads + 2 * kv) * d, dtype=bf16).to(DEV)
+    out, lse, weights = torch.zeros(0, heads * d, dtype=bf16).to(DEV), torch.zeros(0, heads).to(DEV), torch.ones(2, kv, page).to(DEV)
+    hip.qk_norm_rope_store(qkv, i32(0), None, None, None, 1e-6, heads, kv, d, 0, cache, i32(0), page)
+    hip.paged_attention(qkv[:, :heads * d].view(0, heads, d), cache, meta, out, 0.125, lse=lse)
+    hip.attention_weights(qkv[:, :heads * d].view(0, heads, d), cache, meta, lse, weights, 0.125)
+    hip.evict_tokens(cache, weights, i32(0, 1), i32(0), i32(0, 1), 5, 1, i32(0, kv, 5), longest=0)
+    hip.unpack_cache(cache, i32(0), torch.zeros(0, 2, kv, page, d, dtype=bf16).to(DEV))
+    assert not cache.any() and (weights == 1).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("heads,kv,d,page,ctx,new,window", [ATTEND[i] for i in (1, 2, 6, 7, 11, 13)])
 def test_logsum_of_the_engines_own_cache(hip, dtype, heads, kv, d, page, ctx, new, window):
@@ -457,6 +494,31 @@ def test_eviction_of_equal_weights_keeps_the_first(hip):
     assert kept.cpu().flatten().tolist() == list(range(35)) + list(range(85, 90))
 
 
+@pytest.mark.parametrize("kind", ["fp4", "own"])
+def test_eviction_from_a_table_with_pages_given_back(hip, kind):
+    """Tokens whose page is gone go first; where too few others are left, a new place of one stays as it was."""
+    kv, d, page, length, recent = 2, 64, 32, 200, 8
+    for keep in (100, 180):                 # 40 + 96 + 64 tokens, the 64 of two middle pages gone: 136 are left
+        meta, cache, layer, weights, new_table = evict_case(kind, torch.bfloat16, kv, d, page, [length], keep)
+        table = meta.block_table.clone()
+        table[0, 1] = table[0, 4] = -1
+        gone = (torch.arange(length) // page == 1) | (torch.arange(length) // page == 4)
+        got, got_w = cache.clone().to(DEV), weights.clone().to(DEV)
+        kept = torch.empty(1, kv, keep, dtype=torch.int32).to(DEV)
+        hip.evict_tokens(got, got_w, table, torch.tensor([length], dtype=torch.int32).to(DEV), new_table.to(DEV), keep, recent, kept,
+                         longest=length)
+        at, held = torch.arange(length), table.cpu().long()[0].clamp(min=0)
+        for h in range(kv):
+            w = weights[held[at // page], h, at % page].clone()
+            w[gone] = float("-inf")          # below every weight of the case
+            stay = oracle.chosen(w.tolist(), length, keep, recent)
+            assert kept.cpu()[0, h].tolist() == stay
+            for to, i in enumerate(stay):
+                where = (new_table[0, to // page].long(), h, to % page)
+                expected = weights[where] if gone[i] else weights[held[i // page], h, i % page]
+                assert got_w.cpu()[where] == expected
+
+
 # ---------------------------------------------------------------------------------------------- together
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_a_request_in_4_bits_from_store_to_eviction(hip, dtype):
@@ -596,6 +658,14 @@ def test_refusals(hip):
     wrong = type(meta)(**{**vars(meta), "item_q_len": np.asarray([2])})
     with pytest.raises(ValueError):
         weigh(meta=wrong)
+    for items in (dict(item_q_len=np.asarray([2])), dict(item_q_len=np.asarray([0])), dict(item_ctx_len=np.asarray([65])),
+                  dict(item_ctx_len=np.asarray([50, 1]))):
+        with pytest.raises(ValueError):
+            attend(meta=type(meta)(**{**vars(meta), "block_table": meta.block_table[:, :2].contiguous(), "work": {}, **items}))
+    flat = torch.zeros(cache.numel() + 8, dtype=torch.uint8).to(DEV)
+    for call in (attend, weigh):
+        with pytest.raises(KernelShapeError):      # a cache that begins between multiples of 16 bytes
+            call(cache=flat[8:].view(cache.shape))
     short = type(meta)(**{**vars(meta), "block_table": meta.block_table[:, :1].contiguous(), "item_ctx_len": np.asarray([50])})
     with pytest.raises(ValueError):
         weigh(meta=short)

@@ -8,6 +8,7 @@ import torch
 import tests.compact_oracle as oracle
 from sparseengine_amd import LLM, SamplingParams
 from sparseengine_amd.cache import layout
+from sparseengine_amd.kernels import attention_work
 from tests import backends
 from tests.helpers import CONFIGS, make_folder, random_tokens
 from tests.test_gpu_compact_cache import check_attention
@@ -112,7 +113,10 @@ def all_free(llm):
     assert all(g.pool.free_count == g.pool.num_pages for g in cache.groups) and not cache.row_dropped.any()
 
 
-def check_cache_in_4_bits(tmp_path, key, dtype, lengths, new, **kwargs):
+def check_cache_in_4_bits(tmp_path, monkeypatch, key, dtype, lengths, new, blocks=False, **kwargs):
+    """``blocks``: prompts of any length go in blocks, over unpacked pages."""
+    if blocks:
+        monkeypatch.setattr(attention_work, "FP4_BLOCK_WORK", 0)
     folder, prompts = make_folder(tmp_path, key), prompts_for(key, lengths)
     kernels = watched(backends.ACTIVE.kernels())
     llm = engine(folder, kernels, dtype=dtype, kv_cache_dtype="fp4", **kwargs)
@@ -152,12 +156,13 @@ def check_large_budget_changes_nothing(tmp_path, key, dtype, lengths, new, **kwa
 
 
 @pytest.mark.parametrize("key,dtype,lengths,new,kwargs", [
-    ("C_loud", "bfloat16", (1, 33, 70), 5, {}),                                   # the 4-bit kernel, prompts in blocks unpacked
+    ("C_loud", "bfloat16", (1, 33, 70), 5, {}),                                   # the 4-bit kernel
+    ("C_loud", "bfloat16", (1, 33, 70), 5, dict(blocks=True)),                    # and its prompts in unpacked blocks
     ("C_loud", "bfloat16", (90, 8), 4, dict(max_num_batched_tokens=24)),          # portions beside decodes
     ("C_loud", "float32", (40, 3), 4, {}),                                        # unpacked, the general kernel
     ("B_loud", "bfloat16", (40, 3), 4, dict(kv_page_size=64))])                   # a head size without a kernel of its own
-def test_cache_in_4_bits(tmp_path, key, dtype, lengths, new, kwargs):
-    check_cache_in_4_bits(tmp_path, key, dtype, lengths, new, **kwargs)
+def test_cache_in_4_bits(tmp_path, monkeypatch, key, dtype, lengths, new, kwargs):
+    check_cache_in_4_bits(tmp_path, monkeypatch, key, dtype, lengths, new, **kwargs)
 
 
 @pytest.mark.parametrize("key,dtype,lengths,new,budget,recent,kwargs", [
