@@ -78,9 +78,9 @@ attention_weights_generic_kernel(const T* __restrict__ q, int64_t q_stride, cons
 //   S = Q K^T        v_mfma_f32_16x16x32_bf16, A = 16 rows x 32 dims, B = 32 dims x 16 keys, so that a lane ends up
 //                    with four rows of one key and the sum over rows is additions in a lane; the four lanes that
 //                    share a key meet once at the end.
-// With one tile of rows (decoding) a block is four wavefronts side by side along the keys, and the kernel is bound by
-// the chain of loads in front of its few products: the request's lengths, the page ids, the keys (rows and previous
-// weights are on their way with them).  With more, the wavefronts of a block take turns at the tiles of the same
+// With one tile of rows (decoding; in 4 bits most head sizes have the kernel behind this one for it) a block is four
+// wavefronts side by side along the keys, and the kernel is bound by the chain of loads in front of its few products: the
+// request's lengths, the page ids, the keys (rows and previous weights are on their way with them).  With more, the wavefronts of a block take turns at the tiles of the same
 // keys (`row_waves`), and several blocks do where there are too few of them to fill the chip evenly (`row_blocks`:
 // their sums go to a workspace and a second kernel adds them up); everything is added in one order, and the kernel is
 // bound by the exponentials and the products.
@@ -437,6 +437,156 @@ attention_weights_mfma_kernel(const bf16_t* __restrict__ q, int64_t q_stride, co
     }
 }
 
+// The same for one tile of rows (decoding) over a cache in 4 bits at head sizes whose part of a key is one piece to a
+// lane: a wavefront goes through `per_wave` groups of 32 keys with the codes, factors and previous weights of
+// ONE_TILE_DEPTH groups on their way, and turns a group into operands when its turn comes.  Owning 128 keys and ending,
+// as the kernel above does, spends more instructions on finding rows, pages and places than on the keys (16 requests of
+// up to 8200 keys, 48:8 heads of 128: 19 us, now 15.6; 64 of up to 30000 keys 281 us, now 215, 4.1 TB/s of codes, factors
+// and weights, where attention over the same pages reads at 4.6).  The sums of a group's two keys to a lane meet in one
+// pass over the four lanes that share them.  HIDDEN: some request has several tokens, whose rows do not all see the last keys; with a single
+// token a key that it cannot see is one whose weight is not written.
+#define ONE_TILE_DEPTH 4
+template <int DS, bool HIDDEN>
+__global__ void __launch_bounds__(256, 2)
+attention_weights_one_tile_fp4_kernel(const bf16_t* __restrict__ q, int64_t q_stride, const uint8_t* __restrict__ cache,
+                                      const int32_t* __restrict__ block_table, int bt_stride,
+                                      const int32_t* __restrict__ item_meta, int items, int longest,
+                                      const float* __restrict__ lse, const float* previous, float* out, int heads,
+                                      int kv_heads, int page_size, float scale_log2e, int window, int per_wave) {
+  static_assert(DS == 2 || DS == 4 || DS == 8, "a lane's part of a key lies in one piece of memory per group");
+  constexpr int D = 32 * DS, DEPTH = ONE_TILE_DEPTH;
+  constexpr int PIECES = (DS + 3) / 4, WORDS = DS == 2 ? 2 : 4;      // of a lane's part of a key: groups of dims, words of codes
+  const int lane = threadIdx.x & (SE_WAVE - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / SE_WAVE));
+  const int n = lane & 15, g = lane >> 4;
+  const int item = blockIdx.z, kvh = blockIdx.x, group = heads / kv_heads;
+  const int q_start = item_meta[item], q_len = item_meta[items + item], ctx_len = min(item_meta[2 * items + item], longest);
+  const int pos0 = ctx_len - q_len;
+  const int low_key = window > 0 && pos0 - window + 1 > 0 ? pos0 - window + 1 : 0;
+  const int first = low_key / 32 + (static_cast<int>(blockIdx.y) * 4 + wave) * per_wave;      // of the wavefront's groups
+  const int last = min(first + per_wave, (ctx_len + 31) / 32) - 1;
+  if (first > last) return;
+  const int32_t* table = block_table + static_cast<int64_t>(item) * bt_stride;
+
+  // a page's bytes of a group of dims that this lane reads, relative to the group of keys
+  const int64_t head_bytes = fp4_head_bytes(page_size, D), factors = fp4_factors_at(page_size, D);
+  const int dims = DS == 2 ? g >> 1 : g * PIECES;      // its first group of dims
+  const int lane_codes = (dims * page_size + 2 * n) * 16 + (DS == 2 ? (g & 1) * 8 : 0);
+  const int lane_factors = static_cast<int>(factors) + dims * page_size + (2 * n & ~3), half_shift = (n & 1) * 16;
+  const int lane_key = 2 * n + (g >> 1);               // whose weight it reads, and writes if g is even
+  const float* old = previous != nullptr ? previous : out;      // out: read, but not taken
+
+  // the rows: lane (g, n) has dims of row n as an operand, and what belongs to rows 4 g + i
+  const int rows = q_len * group, row = min(n, rows - 1);
+  uint4 rows_q[DS];
+  {
+    const bf16_t* at = q + static_cast<int64_t>(q_start + row / group) * q_stride + static_cast<int64_t>(kvh * group + row % group) * D + (D / 4) * g;
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) rows_q[ds] = *reinterpret_cast<const uint4*>(at + 8 * ds);
+  }
+  float l[4];      // turned into powers of two below; +inf: there is no such row
+  int pos[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = min(4 * g + i, rows - 1), token = r / group;
+    const float of_row = lse[static_cast<int64_t>(q_start + token) * heads + kvh * group + r - token * group];
+    l[i] = of_row;
+    pos[i] = pos0 + token;
+  }
+  // asked for before the keys: a wait for what comes later would be one for them too
+  __builtin_amdgcn_sched_barrier(0);
+
+  se_u32x4 codes[DEPTH][2][PIECES];
+  uint32_t factor[DEPTH][PIECES];      // of two lanes' keys (16 bits would be widened, or packed, where they are waited for)
+  float before[DEPTH];
+  int64_t place[DEPTH];
+  int page = first * 32 / page_size, off = first * 32 - page * page_size, asked = first;
+  const int last_page = last * 32 / page_size;
+  int id = table[page], next_id = table[min(page + 1, last_page)];
+#define ONE_TILE_ASK(S)                                                                                                  \
+  {                                                                                                                      \
+    const uint8_t* at = cache + (static_cast<int64_t>(id) * 2 * kv_heads + kvh) * head_bytes;                            \
+    _Pragma("unroll") for (int h = 0; h < PIECES; ++h) {                                                                 \
+      factor[S][h] = *reinterpret_cast<const uint32_t*>(at + off + lane_factors + h * page_size);                        \
+      _Pragma("unroll") for (int b = 0; b < 2; ++b) {                                                                    \
+        const uint8_t* piece = at + off * 16 + lane_codes + h * page_size * 16 + b * 16;                                 \
+        if constexpr (DS == 2) {                                                                                         \
+          const uint2 v = *reinterpret_cast<const uint2*>(piece);                                                        \
+          codes[S][b][h] = se_u32x4{v.x, v.y, 0, 0};                                                                     \
+        } else {                                                                                                         \
+          codes[S][b][h] = __builtin_nontemporal_load(reinterpret_cast<const se_u32x4*>(piece));                         \
+        }                                                                                                                \
+      }                                                                                                                  \
+    }                                                                                                                    \
+    place[S] = (static_cast<int64_t>(id) * kv_heads + kvh) * page_size + off;                                            \
+    before[S] = old[place[S] + lane_key];                                                                                \
+    if (asked < last) { /* beyond the last group: that one once more */                                                  \
+      ++asked;                                                                                                           \
+      off += 32;                                                                                                         \
+      if (off == page_size) {                                                                                            \
+        off = 0;                                                                                                         \
+        id = next_id;                                                                                                    \
+        ++page;                                                                                                          \
+        next_id = table[min(page + 1, last_page)];                                                                       \
+      }                                                                                                                  \
+    }                                                                                                                    \
+  }
+#pragma unroll
+  for (int s = 0; s < DEPTH; ++s) {
+    ONE_TILE_ASK(s)
+  }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) l[i] = 4 * g + i < rows ? l[i] * 1.4426950408889634f : INFINITY;
+
+#define ONE_TILE_WEIGH(S, AT)                                                                                            \
+  {                                                                                                                      \
+    floatx4 sc[2];                                                                                                       \
+    _Pragma("unroll") for (int b = 0; b < 2; ++b) {                                                                      \
+      sc[b] = floatx4{0.f, 0.f, 0.f, 0.f};                                                                               \
+      _Pragma("unroll") for (int h = 0; h < PIECES; ++h) {                                                               \
+        const uint32_t two = factor[S][h] >> half_shift, f = b == 0 ? fp4_factor_bits<0>(two) : fp4_factor_bits<1>(two); \
+        _Pragma("unroll") for (int w = 0; w < WORDS; ++w)                                                                \
+          sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, rows_q[WORDS * h + w]),             \
+                                                          __builtin_bit_cast(bf16x8, fp4_eight(codes[S][b][h][w], f)),   \
+                                                          sc[b], 0, 0, 0);                                               \
+      }                                                                                                                  \
+    }                                                                                                                    \
+    float sum[2];                                                                                                        \
+    _Pragma("unroll") for (int b = 0; b < 2; ++b) {                                                                      \
+      const int key = 32 * (AT) + 2 * n + b;                                                                             \
+      sum[b] = 0.f;                                                                                                      \
+      _Pragma("unroll") for (int i = 0; i < 4; ++i) {                                                                    \
+        float v = fmaf(sc[b][i], scale_log2e, -l[i]);                                                                    \
+        if (HIDDEN) v = ((key > pos[i]) | (window > 0 & key <= pos[i] - window)) ? -INFINITY : v;                        \
+        sum[b] += __builtin_amdgcn_exp2f(v);                                                                             \
+      }                                                                                                                  \
+    }                                                                                                                    \
+    /* lanes of g = 0, 1 end up with the first key's sum over the four lanes, those of g = 2, 3 with the second's */    \
+    const auto half = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum[0]), __float_as_uint(sum[1]), false, false);  \
+    const float two = __uint_as_float(half[0]) + __uint_as_float(half[1]);                                               \
+    const auto rest = __builtin_amdgcn_permlane16_swap(__float_as_uint(two), __float_as_uint(two), false, false);        \
+    const float total = __uint_as_float(rest[0]) + __uint_as_float(rest[1]);                                             \
+    const int key = 32 * (AT) + lane_key;                                                                                \
+    const float was = previous != nullptr && key < pos0 ? before[S] : 0.f;                                               \
+    if ((AT) <= last && (g & 1) == 0 && key < ctx_len && key >= low_key) out[place[S] + lane_key] = was + total;         \
+  }
+  int at = first;
+  for (; at + DEPTH <= last; at += DEPTH) {      // while groups are left that are not yet on their way
+#pragma unroll
+    for (int s = 0; s < DEPTH; ++s) {
+      ONE_TILE_WEIGH(s, at + s)
+      ONE_TILE_ASK(s)
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < DEPTH; ++s) {
+    ONE_TILE_WEIGH(s, at + s)
+  }
+#undef ONE_TILE_ASK
+#undef ONE_TILE_WEIGH
+}
+
 // Adds up the sums of `row_blocks` blocks of every key.
 __global__ void __launch_bounds__(256)
 join_weights_kernel(const float* __restrict__ partial, int row_blocks, const int32_t* __restrict__ block_table, int bt_stride,
@@ -457,6 +607,9 @@ join_weights_kernel(const float* __restrict__ partial, int row_blocks, const int
 // as a wavefront has at least four tiles (2048 rows x 6 heads on 6000 keys, 8 kv heads: 376 blocks alone run in one
 // round and a half, 241 us).
 #define WEIGHT_BLOCKS 1536
+// Wavefronts of the one-tile kernel: more than run at once (five per SIMD), since requests differ in length (16 x 8200
+// keys: 19 us with 2048, 17.6 with 4096, 15.6 with 16384; 64 x 30000 keys 217 us with any).
+#define ONE_TILE_WAVES 16384
 static int many_rows_keys(int head_dim) {      // of a wavefront, as WeightShape has it
   const int ds = head_dim / 32;
   return 32 * (ds == 1 ? 8 : ds <= 4 ? 4 : ds <= 6 ? 2 : 1);
@@ -479,11 +632,30 @@ extern "C" int se_attention_weights_splits(int items, int longest, int most_new,
 
 template <int DS, int KIND>
 static void launch_weights_mfma(const void* q, int64_t q_stride, const void* cache, const int32_t* block_table, int bt_stride,
-                                const int32_t* item_meta, int items, int longest, int most_rows, const float* lse,
+                                const int32_t* item_meta, int items, int longest, int most_new, const float* lse,
                                 const float* previous, float* out, int heads, int kv_heads, int page_size, float scale,
                                 int window, int splits, float* partial, hipStream_t stream) {
   // With a single tile there is nothing to share out among the wavefronts of the same keys.
-  const int tiles = (most_rows + 15) / 16;
+  const int tiles = static_cast<int>((static_cast<int64_t>(most_new) * (heads / kv_heads) + 15) / 16);
+  constexpr bool ONE_TILE_FP4 = KIND == SE_CACHE_FP4 && (DS == 2 || DS == 4 || DS == 8);
+  if constexpr (ONE_TILE_FP4) {
+    if (tiles <= 1) {
+      // groups of a wavefront, in whole rounds of those on their way
+      const int span = window > 0 && window + most_new + 62 < longest ? window + most_new + 62 : longest;
+      const int64_t groups = (span + 31) / 32, all = groups * kv_heads * items;
+      int per_wave = static_cast<int>((all + ONE_TILE_WAVES - 1) / ONE_TILE_WAVES);
+      per_wave = (per_wave + ONE_TILE_DEPTH - 1) / ONE_TILE_DEPTH * ONE_TILE_DEPTH;
+      const dim3 grid(kv_heads, static_cast<unsigned>((groups + 4 * per_wave - 1) / (4 * per_wave)), items);
+#define SE_WEIGHTS_ONE_TILE(HIDDEN)                                                                                        \
+  attention_weights_one_tile_fp4_kernel<DS, HIDDEN><<<grid, 256, 0, stream>>>(                                             \
+      static_cast<const bf16_t*>(q), q_stride, static_cast<const uint8_t*>(cache), block_table, bt_stride, item_meta, items, longest, \
+      lse, previous, out, heads, kv_heads, page_size, scale * 1.4426950408889634f, window, per_wave)
+      if (most_new > 1) SE_WEIGHTS_ONE_TILE(true);
+      else SE_WEIGHTS_ONE_TILE(false);
+#undef SE_WEIGHTS_ONE_TILE
+      return;
+    }
+  }
 #define SE_WEIGHTS_LAUNCH(MODE, ROW_WAVES, ROW_BLOCKS)                                                                     \
   {                                                                                                                        \
     constexpr int waves = WeightShape<DS, MODE>::WAVES;                                                                    \
@@ -493,8 +665,9 @@ static void launch_weights_mfma(const void* q, int64_t q_stride, const void* cac
         static_cast<const bf16_t*>(q), q_stride, cache, block_table, bt_stride, item_meta, items, longest, lse, previous, out, \
         heads, kv_heads, page_size, scale * 1.4426950408889634f, window, ROW_WAVES, ROW_BLOCKS, partial);                  \
   }
-  if (tiles <= 1) SE_WEIGHTS_LAUNCH(ROWS_ONE, 1, 1)
-  else if (tiles <= 8) SE_WEIGHTS_LAUNCH(ROWS_FEW, 2, 1)
+  if (tiles <= 1) {
+    if constexpr (!ONE_TILE_FP4) SE_WEIGHTS_LAUNCH(ROWS_ONE, 1, 1)
+  } else if (tiles <= 8) SE_WEIGHTS_LAUNCH(ROWS_FEW, 2, 1)
   else if (tiles <= 32) SE_WEIGHTS_LAUNCH(ROWS_FEW, 4, 1)
   else SE_WEIGHTS_LAUNCH(ROWS_MANY, waves, splits)
 #undef SE_WEIGHTS_LAUNCH
@@ -523,7 +696,7 @@ extern "C" int se_attention_weights(const void* q, int64_t q_stride, const void*
     if (splits > 1 && workspace == nullptr) return SE_ERR_SHAPE;
 #define SE_WEIGHTS_MFMA(DS, KIND)                                                                                   \
   launch_weights_mfma<DS, KIND>(q, q_stride, cache, block_table, bt_stride, item_meta, items, longest,              \
-                                static_cast<int>(most_rows), lse, previous, out, heads, kv_heads, page_size, scale, window, splits, workspace, stream)
+                                most_new, lse, previous, out, heads, kv_heads, page_size, scale, window, splits, workspace, stream)
 #define SE_WEIGHTS_CASE(DS)                                     \
   case DS:                                                      \
     if (kind == SE_CACHE_FP4) SE_WEIGHTS_MFMA(DS, SE_CACHE_FP4); \
