@@ -16,36 +16,44 @@
 enum SeCacheKind { SE_CACHE_F32 = 0, SE_CACHE_BF16 = 1, SE_CACHE_FP4 = 2 };
 
 // General form, any head size in steps of 8 and any kind of cache (the float path of the engine, and sizes that the
-// matrix-core kernel does not take): a lane owns a key, and reads it again for every row.
+// matrix-core kernel does not take): a lane owns a key, four wavefronts share the rows of 64 keys, four rows at a time so
+// that a key is read once for four.  Bound by the latency of a few such rounds where rows are few (3 requests of up to
+// 300 keys with 5 new tokens each, 12:2 heads of 64 in float32: 9 us; row by row in one wavefront 24 us).
+#define GENERIC_WAVES 4
+#define GENERIC_ROWS 4
 template <typename T, int KIND>
-__global__ void __launch_bounds__(64)
+__global__ void __launch_bounds__(GENERIC_WAVES * SE_WAVE)
 attention_weights_generic_kernel(const T* __restrict__ q, int64_t q_stride, const void* __restrict__ cache,
                                  const int32_t* __restrict__ block_table, int bt_stride,
                                  const int32_t* __restrict__ item_meta, int items, int longest,
                                  const float* __restrict__ lse, const float* previous, float* out, int heads, int kv_heads, int head_dim,
                                  int page_size, float scale, int window) {
-  extern __shared__ float q_row[];     // [head_dim]
+  extern __shared__ float q_rows[];     // [GENERIC_WAVES][GENERIC_ROWS][head_dim]
+  __shared__ float sums[GENERIC_WAVES][SE_WAVE];
   const int item = blockIdx.z, kvh = blockIdx.y, group = heads / kv_heads;
+  const int lane = threadIdx.x & (SE_WAVE - 1), wave = threadIdx.x / SE_WAVE;
   const int q_start = item_meta[item], q_len = item_meta[items + item], ctx_len = min(item_meta[2 * items + item], longest);
-  const int pos0 = ctx_len - q_len;
+  const int pos0 = ctx_len - q_len, rows = q_len * group;
   const int low_key = window > 0 && pos0 - window + 1 > 0 ? pos0 - window + 1 : 0;   // no row sees a key before it
   const int base = blockIdx.x * SE_WAVE;
   if (base >= ctx_len || base + SE_WAVE <= low_key) return;
-  const int key = base + threadIdx.x;
+  const int key = base + lane;
   const bool held = key < ctx_len && key >= low_key;
   const int page = held ? block_table[static_cast<int64_t>(item) * bt_stride + key / page_size] : 0;
   const int off = key % page_size;
+  float* mine = q_rows + wave * GENERIC_ROWS * head_dim;
   float total = 0.f;
-  for (int rho = 0; rho < q_len * group; ++rho) {
-    const int pos = pos0 + rho / group;
-    if (pos < base || (window > 0 && pos - window >= base + SE_WAVE - 1)) continue;     // sees none of the 64 keys
-    const int token = q_start + rho / group, head = kvh * group + rho % group;
-    __syncthreads();
-    for (int d = threadIdx.x; d < head_dim; d += SE_WAVE)
-      q_row[d] = to_float(q[token * q_stride + static_cast<int64_t>(head) * head_dim + d]);
-    __syncthreads();
-    if (!held || key > pos || (window > 0 && key <= pos - window)) continue;
-    float dot = 0.f;
+  // rows of tokens before the first key see none of the 64
+  for (int rho = max(0, base - pos0) * group + wave * GENERIC_ROWS; rho < rows; rho += GENERIC_WAVES * GENERIC_ROWS) {
+    if (window > 0 && pos0 + rho / group - window >= base + SE_WAVE - 1) break;     // nor do this one and all after it
+    __builtin_amdgcn_wave_barrier();      // (a wavefront's own accesses to shared memory stay in their order)
+    for (int i = lane; i < GENERIC_ROWS * head_dim; i += SE_WAVE) {
+      const int row = min(rho + i / head_dim, rows - 1);
+      mine[i] = to_float(q[(q_start + row / group) * q_stride + static_cast<int64_t>(kvh * group + row % group) * head_dim + i % head_dim]);
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (!held) continue;
+    float dot[GENERIC_ROWS] = {0.f, 0.f, 0.f, 0.f};
     if constexpr (KIND == SE_CACHE_FP4) {
       const uint8_t* part = static_cast<const uint8_t*>(cache) +
                             (static_cast<int64_t>(page) * 2 * kv_heads + kvh) * fp4_head_bytes(page_size, head_dim);
@@ -53,7 +61,11 @@ attention_weights_generic_kernel(const T* __restrict__ q, int64_t q_stride, cons
         const uint32_t word = *reinterpret_cast<const uint32_t*>(part + fp4_key_code_at(page_size, off, d / 32) + d % 32 / 2);
         const int factor = part[fp4_key_factor_at(page_size, head_dim, off, d / 32)];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) dot += q_row[d + j] * fp4_value(word >> (4 * j) & 15u, factor);
+        for (int j = 0; j < 8; ++j) {
+          const float k = fp4_value(word >> (4 * j) & 15u, factor);
+#pragma unroll
+          for (int r = 0; r < GENERIC_ROWS; ++r) dot[r] += mine[r * head_dim + d + j] * k;
+        }
       }
     } else {
       typedef typename std::conditional<KIND == SE_CACHE_F32, float, bf16_t>::type C;
@@ -62,12 +74,24 @@ attention_weights_generic_kernel(const T* __restrict__ q, int64_t q_stride, cons
         Vec16<C> k;
         k.v = *reinterpret_cast<const decltype(k.v)*>(part + key_place(page_size, off, d));
 #pragma unroll
-        for (int j = 0; j < Vec16<C>::N; ++j) dot += q_row[d + j] * k.get(j);
+        for (int j = 0; j < Vec16<C>::N; ++j) {
+#pragma unroll
+          for (int r = 0; r < GENERIC_ROWS; ++r) dot[r] += mine[r * head_dim + d + j] * k.get(j);
+        }
       }
     }
-    total += expf(dot * scale - lse[static_cast<int64_t>(token) * heads + head]);
+#pragma unroll
+    for (int r = 0; r < GENERIC_ROWS; ++r) {
+      const int row = rho + r, pos = pos0 + row / group;
+      if (row >= rows || key > pos || (window > 0 && key <= pos - window)) continue;
+      total += expf(dot[r] * scale - lse[static_cast<int64_t>(q_start + row / group) * heads + kvh * group + row % group]);
+    }
   }
-  if (!held) return;
+  sums[wave][lane] = total;
+  __syncthreads();
+  if (wave != 0 || !held) return;
+#pragma unroll
+  for (int w = 1; w < GENERIC_WAVES; ++w) total += sums[w][lane];
   const int64_t at = (static_cast<int64_t>(page) * kv_heads + kvh) * page_size + off;
   out[at] = (previous != nullptr && key < pos0 ? previous[at] : 0.f) + total;
 }
@@ -712,9 +736,9 @@ extern "C" int se_attention_weights(const void* q, int64_t q_stride, const void*
     return SE_OK;
   }
   const dim3 grid((longest + SE_WAVE - 1) / SE_WAVE, kv_heads, items);
-  const size_t shared = static_cast<size_t>(head_dim) * sizeof(float);
+  const size_t shared = static_cast<size_t>(GENERIC_WAVES * GENERIC_ROWS) * head_dim * sizeof(float);      // 32 KB at most
 #define SE_WEIGHTS(T, KIND)                                                                                      \
-  attention_weights_generic_kernel<T, KIND><<<grid, 64, shared, stream>>>(                                       \
+  attention_weights_generic_kernel<T, KIND><<<grid, GENERIC_WAVES * SE_WAVE, shared, stream>>>(                  \
       static_cast<const T*>(q), q_stride, cache, block_table, bt_stride, item_meta, items, longest, lse, previous, out, heads, \
       kv_heads, head_dim, page_size, scale, window)
   if (dtype == SE_F32) {

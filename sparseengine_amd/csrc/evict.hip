@@ -8,7 +8,11 @@
 //            that the crowd of words with one exponent does not queue up at one address); the search ends early when
 //            the words at or above the one found are just those wanted, and among words equal to the smallest the
 //            first are kept.  Whole numbers only: the result does not depend on the order in which threads count.
-//   move     the chosen tokens' keys, values, factors and weights, gathered into the new pages.
+//            One block's chain of passes: 2048 of 2112 tokens 12 us, 8192 of 32768 tokens 40 us, whatever the heads.
+//   move     the chosen tokens' keys, values, factors and weights, gathered into the new pages.  Bound by reading: tokens
+//            lie in groups of eight in a page, so that a fourth of the tokens, chosen here and there, touches nearly
+//            every line of the old pages (4 requests, 8192 of 32768 tokens, bfloat16, 8 heads of 128: 126 us for 537 MB
+//            touched and 134 MB written, 5.3 TB/s; 8 requests, 2048 of 2112 tokens in 4 bits: 14 us).
 //
 // `weights` lies in pages beside the cache: [pages, kv_heads, page_size] float.  The new pages must not be among the
 // requests' old ones: the old are read while the new are written.

@@ -554,7 +554,7 @@ class HipKernels:
         goes in here; ``meta`` needs its items.  ``out`` and ``previous``: float32 ``[pages, kv_heads, page_size]`` in
         the cache's pages; they may be the same tensor.  ``previous`` counts for the keys that are older than the
         step (None: nothing for them either); the step's own keys begin with 0.  Keys that no row can see (a window)
-        are left as they are."""
+        are left as they are.  No two items share a page."""
         tokens, heads, head_dim = q.shape
         fp4 = cache.dtype == torch.uint8
         _require(q.stride(2) == 1 and q.stride(1) == head_dim, "q heads must be dense")
@@ -660,7 +660,9 @@ class HipKernels:
         ``out``: ``[T, heads * head_dim]``; ``lse``: None, or float32 ``[T, heads]`` that receives every row's
         logarithm of its sum of exponentials.  A uint8 ``cache`` holds keys and values in 4 bits (``[pages, 2, kv_heads,
         page_size, head_dim * 17 / 32]``, cache/layout.py): ``meta`` then needs its items, ``scale`` is positive, and
-        the call allocates what its longer way needs."""
+        the call allocates what its longer way needs: partial results, and for the portions of prompts that it reads
+        through unpacked pages a copy of those in ``q``'s type.  (There, as over the engine's own cache, a value that is
+        not a number reaches the rows of earlier tokens in its block too.)"""
         tokens, heads, head_dim = q.shape
         kv_heads, page_size = cache.shape[2], cache.shape[3]
         _require(q.stride(2) == 1 and q.stride(1) == head_dim, "q heads must be dense")
