@@ -188,3 +188,15 @@ def test_more_tokens_than_the_cache_has_room_for(tmp_path):
         run(engine(folder, dtype="float32", kv_page_size=16, num_kvcache_slots=96), prompts, 50)
     assert [len(o) for o in run(llm, prompts, 50)] == [50, 50] and llm.method.evictions > 2
     all_free(llm)
+
+
+def test_the_engines_own_choice_of_how_much_cache(tmp_path):
+    """Without a number of cache slots: what the memory holds, or what so many requests of full length could use."""
+    folder, prompts = make_folder(tmp_path, "C_loud"), prompts_for("C_loud", (70, 9))
+    kwargs = dict(dtype="bfloat16", num_kvcache_slots=None, max_num_seqs_in_gpu=4, kv_cache_dtype="fp4", gpu_memory_utilization=0.9)
+    llm = engine(folder, **kwargs)
+    assert llm.runner.cache.groups[0].pool.num_pages * 32 >= llm.config.max_model_len * 4 or backends.ACTIVE.name == "hip"
+    evicting = engine(folder, sparse_method="accumulated_weight", eviction_budget=40, **kwargs)
+    assert run(llm, prompts, 3) and run(evicting, prompts, 3) and evicting.method.evictions > 0
+    all_free(llm)
+    all_free(evicting)
