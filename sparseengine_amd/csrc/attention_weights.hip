@@ -642,6 +642,7 @@ static bool weights_on_matrix_cores(int head_dim, int64_t most_rows, int dtype) 
   return dtype == SE_BF16 && head_dim % 32 == 0 && head_dim <= 256 && most_rows < 0x40000000;
 }
 // How many sums of every key a call leaves in its workspace: float [that, items, kv_heads, longest] (1: none is used).
+// Up to 32 tiles of rows it is 1 (the callers rely on it).
 extern "C" int se_attention_weights_splits(int items, int longest, int most_new, int heads, int kv_heads, int head_dim, int dtype) {
   if (items <= 0 || longest <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0) return 1;
   const int64_t most_rows = static_cast<int64_t>(most_new) * (heads / kv_heads);

@@ -12,7 +12,7 @@
 //   move     the chosen tokens' keys, values, factors and weights, gathered into the new pages.  Bound by reading: tokens
 //            lie in groups of eight in a page, so that a fourth of the tokens, chosen here and there, touches nearly
 //            every line of the old pages (4 requests, 8192 of 32768 tokens, bfloat16, 8 heads of 128: 126 us for 537 MB
-//            touched and 134 MB written, 5.3 TB/s; 8 requests, 2048 of 2112 tokens in 4 bits: 14 us).
+//            touched and 134 MB written, 5.3 TB/s; 8 requests, 2048 of 2112 tokens in 4 bits: 12.6 us).
 //
 // `weights` lies in pages beside the cache: [pages, kv_heads, page_size] float.  The new pages must not be among the
 // requests' old ones: the old are read while the new are written.
@@ -257,13 +257,13 @@ move_tokens_kernel(E* cache, float* weights, const int32_t* __restrict__ block_t
   }
 }
 
-// The same for the 4-bit cache: codes and factors are moved as they are.
+// The same for the 4-bit cache, keys and values in one block: codes and factors are moved as they are.
 __global__ void __launch_bounds__(256)
 move_tokens_fp4_kernel(uint8_t* cache, float* weights, const int32_t* __restrict__ block_table, int bt_stride,
                        const int32_t* __restrict__ new_table, int new_stride, const int32_t* __restrict__ kept,
                        int kv_heads, int page_size, int head_dim, int keep) {
-  extern __shared__ int places[];
-  const int item = blockIdx.z >> 1, which = blockIdx.z & 1, kvh = blockIdx.y;
+  extern __shared__ int places[];       // as above; then six numbers for every eight tokens
+  const int item = blockIdx.z, kvh = blockIdx.y;
   const int32_t* table = block_table + static_cast<int64_t>(item) * bt_stride;
   const int32_t* mine = kept + (static_cast<int64_t>(item) * kv_heads + kvh) * keep;
   const int to_page = new_table[static_cast<int64_t>(item) * new_stride + blockIdx.x];
@@ -273,28 +273,74 @@ move_tokens_fp4_kernel(uint8_t* cache, float* weights, const int32_t* __restrict
     const OldPlace from = old_place(table, mine, base + t, keep, page_size);
     places[2 * t] = from.page;
     places[2 * t + 1] = from.off;
-    if (which == 0 && from.page >= 0)
+    if (from.page >= 0)
       weights[(static_cast<int64_t>(to_page) * kv_heads + kvh) * page_size + t] =
           weights[(static_cast<int64_t>(from.page) * kv_heads + kvh) * page_size + from.off];
   }
   __syncthreads();
   const int groups = head_dim / FP4_GROUP;
   const int64_t span = fp4_head_bytes(page_size, head_dim);
-  auto part = [&](int page) { return cache + ((static_cast<int64_t>(page) * 2 + which) * kv_heads + kvh) * span; };
-  uint8_t* dst = part(to_page);
+  auto part = [&](int page, int which) { return cache + ((static_cast<int64_t>(page) * 2 + which) * kv_heads + kvh) * span; };
+  // Values are moved in pieces of eight neighbouring keys' bytes, of codes (16 * groups of them to eight keys) and then of
+  // factors (groups).  Where most tokens stay, the eight come from one or two pieces of the old pages, whose words are
+  // read whole; else byte by byte.  (8 x 2048 of 2112 tokens: 15 us with all values byte by byte and keys and values in
+  // blocks of their own, 12.6 so.)
+  // Of every eight tokens: page and eight of the first and of the last, from which of the two each byte comes (bit 3 of
+  // four) and where it lies there (bits 0 to 2), and whether there are eight (1), from those two only (2).
+  int* eights = places + 2 * page_size;
+  for (int e = threadIdx.x; e < page_size / 8; e += blockDim.x) {
+    const int* from = places + 16 * e;
+    int flags = 3, select = 0;
+    for (int t = 0; t < 8; ++t) {
+      const bool first = from[2 * t] == from[0] && from[2 * t + 1] >> 3 == from[1] >> 3;
+      const bool last = from[2 * t] == from[14] && from[2 * t + 1] >> 3 == from[15] >> 3;
+      if (from[2 * t] < 0) flags = 0;
+      if (!first && !last) flags &= 1;
+      select |= ((first ? 0 : 8) | (from[2 * t + 1] & 7)) << (4 * t);
+    }
+    int* to = eights + 6 * e;
+    to[0] = from[0], to[1] = from[1] >> 3, to[2] = from[14], to[3] = from[15] >> 3, to[4] = select, to[5] = flags;
+  }
+  uint8_t* new_keys = part(to_page, 0);
   for (int i = threadIdx.x; i < page_size * groups; i += blockDim.x) {
     const int group = i / page_size, t = i % page_size;
     if (places[2 * t] < 0) continue;
-    const uint8_t* src = part(places[2 * t]);
+    const uint8_t* src = part(places[2 * t], 0);
     const int off = places[2 * t + 1];
-    if (which == 0) {
-      *reinterpret_cast<uint4*>(dst + fp4_key_code_at(page_size, t, group)) =
-          *reinterpret_cast<const uint4*>(src + fp4_key_code_at(page_size, off, group));
-      dst[fp4_key_factor_at(page_size, head_dim, t, group)] = src[fp4_key_factor_at(page_size, head_dim, off, group)];
+    *reinterpret_cast<uint4*>(new_keys + fp4_key_code_at(page_size, t, group)) =
+        *reinterpret_cast<const uint4*>(src + fp4_key_code_at(page_size, off, group));
+    new_keys[fp4_key_factor_at(page_size, head_dim, t, group)] = src[fp4_key_factor_at(page_size, head_dim, off, group)];
+  }
+  __syncthreads();
+  const int code_pieces = page_size / 8 * 16 * groups, pieces = code_pieces + page_size / 8 * groups;
+  for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
+    const bool code = i < code_pieces;
+    const int per_eight = code ? 16 * groups : groups, at = code ? i : i - code_pieces;
+    const int e = at / per_eight, rest = at - e * per_eight;
+    const int64_t start = code ? 0 : fp4_factors_at(page_size, head_dim);
+    auto piece = [&](int page, int eight) { return reinterpret_cast<const uint64_t*>(part(page, 1) + start) + eight * per_eight + rest; };
+    uint64_t* to = reinterpret_cast<uint64_t*>(part(to_page, 1) + start) + at;
+    const int* of = eights + 6 * e;
+    const uint32_t select = static_cast<uint32_t>(of[4]);
+    if (of[5] == 3) {
+      const uint64_t first = *piece(of[0], of[1]), last = *piece(of[2], of[3]);
+      uint64_t word = 0;
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        word |= ((select >> (4 * t) & 8u ? last : first) >> (8 * (select >> (4 * t) & 7u)) & 255u) << (8 * t);
+      *to = word;
+      continue;
+    }
+    const int* from = places + 16 * e;
+    auto byte_of = [&](int t) { return reinterpret_cast<const uint8_t*>(piece(from[2 * t], from[2 * t + 1] >> 3))[select >> (4 * t) & 7u]; };
+    if (of[5] == 1) {
+      uint64_t word = 0;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) word |= static_cast<uint64_t>(byte_of(t)) << (8 * t);
+      *to = word;
     } else {
-      for (int j = 0; j < 16; ++j)
-        dst[fp4_value_code_at(head_dim, t, group, j)] = src[fp4_value_code_at(head_dim, off, group, j)];
-      dst[fp4_value_factor_at(page_size, head_dim, t, group)] = src[fp4_value_factor_at(page_size, head_dim, off, group)];
+      for (int t = 0; t < 8; ++t)
+        if (from[2 * t] >= 0) reinterpret_cast<uint8_t*>(to)[t] = byte_of(t);
     }
   }
 }
@@ -316,7 +362,7 @@ extern "C" int se_evict_tokens(void* cache, int kind, float* weights, const int3
   else SE_CHOOSE(32);      // more than 32768 tokens: the rest is read again in every pass
 #undef SE_CHOOSE
   SE_CHECK_LAUNCH();
-  const dim3 grid((keep + page_size - 1) / page_size, kv_heads, items * 2);
+  const dim3 grid((keep + page_size - 1) / page_size, kv_heads, kind == 2 ? items : items * 2);
   const size_t shared = static_cast<size_t>(page_size) * 2 * sizeof(int);
   if (kind == 0)
     move_tokens_kernel<float><<<grid, 256, shared, stream>>>(static_cast<float*>(cache), weights, block_table, bt_stride,
@@ -325,7 +371,7 @@ extern "C" int se_evict_tokens(void* cache, int kind, float* weights, const int3
     move_tokens_kernel<uint16_t><<<grid, 256, shared, stream>>>(static_cast<uint16_t*>(cache), weights, block_table, bt_stride,
                                                                 new_table, new_stride, kept, kv_heads, page_size, head_dim, keep);
   else if (kind == 2)
-    move_tokens_fp4_kernel<<<grid, 256, shared, stream>>>(static_cast<uint8_t*>(cache), weights, block_table, bt_stride,
+    move_tokens_fp4_kernel<<<grid, 256, shared + static_cast<size_t>(page_size / 8) * 6 * sizeof(int), stream>>>(static_cast<uint8_t*>(cache), weights, block_table, bt_stride,
                                                           new_table, new_stride, kept, kv_heads, page_size, head_dim, keep);
   else
     return SE_ERR_SHAPE;

@@ -582,8 +582,8 @@ class HipKernels:
         items, longest, most_new, item_meta = self._items(meta, tokens, page)
         _same_device(q, cache, lse, out, previous, meta.block_table, item_meta)
         # sums of several blocks for the same keys (many rows) meet in a workspace of this call's own
-        splits = _fn.get("attention_weights", "se_attention_weights_splits")(items, longest, most_new, heads, kv_heads,
-                                                                             head_dim, _code(q.dtype))
+        splits = 1 if most_new * heads <= 512 * kv_heads else _fn.get("attention_weights", "se_attention_weights_splits")(
+            items, longest, most_new, heads, kv_heads, head_dim, _code(q.dtype))      # 512 rows: one block of them
         workspace = (torch.empty(splits, items, kv_heads, longest, dtype=torch.float32, device=q.device) if splits > 1 else None)
         _check(_fn.get("attention_weights", "se_attention_weights")(
             _ptr(q), q.stride(0), _ptr(cache), self._CACHE_KINDS[cache.dtype], _ptr(meta.block_table),
@@ -596,10 +596,14 @@ class HipKernels:
         if getattr(meta, "item_q_len", None) is None:
             raise ValueError(f"{what} needs the step's items (item_q_len, item_ctx_len)")
         q_len, ctx_len = np.asarray(meta.item_q_len), np.asarray(meta.item_ctx_len)
-        _require(q_len.size == ctx_len.size and q_len.size <= meta.block_table.shape[0] and bool((q_len >= 1).all())
-                 and bool((q_len <= ctx_len).all()) and int(q_len.sum()) == tokens,
+        _require(q_len.size == ctx_len.size and q_len.size <= meta.block_table.shape[0], "items: one context to an item, a block table row each")
+        if q_len.size <= 64:      # a few numbers: five passes over an array cost more than the loop
+            new, held = q_len.tolist(), ctx_len.tolist()
+            right, total, longest = all(1 <= n <= m for n, m in zip(new, held)), sum(new), max(held, default=0)
+        else:
+            right, total, longest = bool((q_len >= 1).all() and (q_len <= ctx_len).all()), int(q_len.sum()), int(ctx_len.max())
+        _require(right and total == tokens,
                  "items: every item needs at least one new token and no more than its context, together the step's tokens")
-        longest = int(ctx_len.max()) if q_len.size else 0
         _require(longest <= meta.block_table.shape[1] * page, "the block table has too few columns for the longest item")
         return q_len, ctx_len, longest
 
