@@ -298,7 +298,8 @@ def test_attention_of_many_rows_in_unpacked_blocks(hip, monkeypatch, heads, kv, 
     assert attention_work.build_fp4_attention_work(new, ctx, heads // kv, kv, window, d).block_units.size
 
 
-@pytest.mark.parametrize("new,ctx", [([1, 170], [300, 4200]), ([700], [700]), ([200, 3, 40], [1200, 40, 5000])])
+@pytest.mark.parametrize("new,ctx", [([1, 170], [300, 4200]), ([700], [700]), ([200, 3, 40], [1200, 40, 5000]),
+                                     ([90, 1], [9000, 20000]), ([1] * 70, list(range(400, 1100, 10)))])      # many rows to join
 def test_portions_around_the_choice_of_a_kernel(hip, new, ctx):
     heads, kv, d, page = 12, 2, 64, 64
     emulator_skips(sum(c * n for c, n in zip(ctx, new)) * heads * d)
