@@ -1,17 +1,21 @@
 """The engine with its cache in 4 bits and with eviction, on the CPU through the kernel sources (a short version of
 tests/test_gpu_compact_engine.py), and what their options refuse."""
+import random
+
 import numpy as np
 import pytest
 import torch
 
 import tests.test_gpu_compact_engine as E
+from sparseengine_amd import LLM, SamplingParams
 from sparseengine_amd.cache.manager import CacheManager
 from sparseengine_amd.cache.page_pool import OutOfPages
 from sparseengine_amd.config.runtime import Config
 from sparseengine_amd.engine.eviction import AccumulatedWeightMethod
 from sparseengine_amd.parts.base import PagedKVRequest
 from tests import backends
-from tests.helpers import make_folder
+from tests.helpers import make_folder, random_tokens
+from tests.twin_kernels import TwinKernels
 
 emulated = pytest.mark.skipif(not backends.EmulatedBackend().available(), reason="no host compiler for the emulated kernels")
 
@@ -105,3 +109,33 @@ def test_the_method_refuses_windows_and_other_head_sizes():
     never = AccumulatedWeightMethod(190, 2, 16)
     never.bind(manager())
     assert never.reserved_pages() == {} and np.asarray(never.weights[0].shape).tolist() == [8, 2, 32]
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_random_requests_under_eviction(tmp_path, seed):
+    """Whatever the sizes, a cache that holds one request and its cut serves all of them: the host's account alone, on
+    twins that evict nothing."""
+    class Twins(TwinKernels):
+        def paged_attention(self, q, cache, meta, out, scale, window=0, lse=None):
+            super().paged_attention(q, cache, meta, out, scale, window)
+
+        def attention_weights(self, *args, **kwargs):
+            pass
+
+        def evict_tokens(self, cache, weights, table, lengths, new_table, keep, recent, kept, longest):
+            assert bool((lengths > keep).all()) and int(lengths.max()) == longest <= table.shape[1] * cache.shape[3]
+            for old, new, n in zip(table.tolist(), new_table.tolist(), lengths.tolist()):
+                assert min(old[:-(-n // cache.shape[3])] + new) >= 0 and not set(old) & set(new) and len(set(new)) == len(new)
+
+    rng = random.Random(seed)
+    page, budget, chunk, most = rng.choice([8, 16, 32]), rng.randint(1, 80), rng.choice([4, 16, 33]), rng.choice([8, 16, 64])
+    one = -(-(budget + page - 1 + min(chunk, most)) // page) + -(-budget // page)      # pages of a request and of its cut
+    llm = LLM(make_folder(tmp_path, "A_loud"), _kernels=Twins(), _device="cpu", dtype="float32", kv_page_size=page,
+              num_kvcache_slots=page * (one + rng.randint(0, 6)), max_num_seqs_in_batch=rng.choice([2, 4, 8]), max_num_batched_tokens=most,
+              engine_prefill_chunk_size=chunk, decode_reservation_tokens=rng.choice([0, 4, 64]), sparse_method="accumulated_weight",
+              eviction_budget=budget, eviction_recent=rng.randint(0, budget), validate_runtime_invariants=True)
+    prompts = [random_tokens(rng.randint(1, 150), 512, seed * 100 + i) for i in range(6)]
+    params = [SamplingParams(temperature=0.0, max_tokens=rng.randint(1, 60), ignore_eos=True) for _ in prompts]
+    out = llm.generate(prompts, params, use_tqdm=False)
+    assert [len(o["token_ids"]) for o in out] == [p.max_tokens for p in params]
+    E.all_free(llm)
