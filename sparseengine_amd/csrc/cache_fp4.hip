@@ -71,7 +71,10 @@ __device__ __forceinline__ void put8(T* dst, const float (&x)[8]) {
 // engine's own cache (key_place, value_place).  Which page: pages[blockIdx.x], or, with a list of (row, column)
 // pairs, the block table's entry there; a negative page is left out.  A thread makes eight elements of a key, or
 // the eight keys of a group for two neighbouring dims of the values.
-template <typename T>
+// FOR_PRODUCTS: for kernels that multiply the probabilities of many rows with a token's values, those of rows that do not
+// see it (0) among them.  A group of values that is not a number is then written as zeros and its token's key as not a number:
+// rows that see the token become so as a whole, the others take nothing from it.
+template <typename T, bool FOR_PRODUCTS>
 __global__ void __launch_bounds__(256)
 fp4_unpack_kernel(const uint8_t* __restrict__ cache, const int32_t* __restrict__ pages, int bt_stride,
                   const int2* __restrict__ list, T* __restrict__ out, int kv_heads, int page_size, int head_dim) {
@@ -92,6 +95,11 @@ fp4_unpack_kernel(const uint8_t* __restrict__ cache, const int32_t* __restrict__
       float x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = fp4_value(word >> (4 * j) & 15u, factor);
+      if (FOR_PRODUCTS && d8 == 0) {
+        const uint8_t* values = part + kv_heads * fp4_head_bytes(page_size, head_dim);
+        for (int group = 0; group < groups; ++group)
+          if (values[fp4_value_factor_at(page_size, head_dim, off, group)] == FP4_NAN) x[0] = __uint_as_float(0x7fc00000u);
+      }
       put8(dst + static_cast<int64_t>(i) * 8, x);             // [head_dim / 8][page_size][8]
     }
   } else {
@@ -106,8 +114,9 @@ fp4_unpack_kernel(const uint8_t* __restrict__ cache, const int32_t* __restrict__
       for (int k = 0; k < 8; ++k) {
         const uint32_t two = (k < 4 ? codes.x : codes.y) >> (k % 4 * 8);
         const int factor = static_cast<int>((k < 4 ? factors.x : factors.y) >> (k % 4 * 8) & 255u);
-        even[k] = fp4_value(two & 15u, factor);
-        odd[k] = fp4_value(two >> 4 & 15u, factor);
+        const bool nothing = FOR_PRODUCTS && factor == FP4_NAN;
+        even[k] = nothing ? 0.f : fp4_value(two & 15u, factor);
+        odd[k] = nothing ? 0.f : fp4_value(two >> 4 & 15u, factor);
       }
       T* at = dst + (static_cast<int64_t>(kg) * head_dim + 2 * pair) * 8;   // [page_size / 8][head_dim][8]
       put8(at, even);
@@ -141,18 +150,20 @@ extern "C" int se_fp4_store(const void* qkv, int64_t row_stride, const int32_t* 
 
 // pages: [count]; or, with `list` (int32 [count, 2]: row, column), a block table with rows of `bt_stride` entries.
 extern "C" int se_fp4_unpack(const void* cache, const int32_t* pages, int bt_stride, const int32_t* list, int count,
-                             void* out, int kv_heads, int page_size, int head_dim, int dtype, hipStream_t stream) {
+                             void* out, int kv_heads, int page_size, int head_dim, int dtype, int for_products, hipStream_t stream) {
   if (count <= 0) return SE_OK;
   if (!fp4_sizes_taken(kv_heads, head_dim, page_size) || 2 * kv_heads > 65535) return SE_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>(count), static_cast<unsigned>(2 * kv_heads));
-  if (dtype == SE_F32)
-    fp4_unpack_kernel<float><<<grid, 256, 0, stream>>>(static_cast<const uint8_t*>(cache), pages, bt_stride, reinterpret_cast<const int2*>(list),
-                                                       static_cast<float*>(out), kv_heads, page_size, head_dim);
-  else if (dtype == SE_BF16)
-    fp4_unpack_kernel<bf16_t><<<grid, 256, 0, stream>>>(static_cast<const uint8_t*>(cache), pages, bt_stride, reinterpret_cast<const int2*>(list),
-                                                        static_cast<bf16_t*>(out), kv_heads, page_size, head_dim);
+#define SE_UNPACK(T, FOR_PRODUCTS)                                                                                      \
+  fp4_unpack_kernel<T, FOR_PRODUCTS><<<grid, 256, 0, stream>>>(static_cast<const uint8_t*>(cache), pages, bt_stride,     \
+                                                               reinterpret_cast<const int2*>(list), static_cast<T*>(out), \
+                                                               kv_heads, page_size, head_dim)
+  if (dtype == SE_F32 && !for_products) SE_UNPACK(float, false);
+  else if (dtype == SE_BF16 && for_products) SE_UNPACK(bf16_t, true);
+  else if (dtype == SE_BF16) SE_UNPACK(bf16_t, false);
   else
     return SE_ERR_SHAPE;
+#undef SE_UNPACK
   SE_CHECK_LAUNCH();
   return SE_OK;
 }

@@ -112,7 +112,7 @@ _SIGNATURES = {
         # qkv, row_stride, slots, tokens, heads, kv_heads, head_dim, cache, page_size, dtype, stream
         "se_fp4_store": [c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p],
         # cache, pages, bt_stride, list, count, out, kv_heads, page_size, head_dim, dtype, stream
-        "se_fp4_unpack": [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
+        "se_fp4_unpack": [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
     },
     "attention_weights": {
         # q, q_stride, cache, kind, block_table, bt_stride, item_meta, items, longest, most_new, lse, previous, out,
@@ -495,7 +495,7 @@ class HipKernels:
             raise KernelShapeError("unpack_cache: out has to begin on a multiple of 16 bytes")
         _check(_fn.get("cache_fp4", "se_fp4_unpack")(
             _ptr(cache), _ptr(pages), 0, None, pages.numel(), _ptr(out), cache.shape[2], page, out.shape[4],
-            _code(out.dtype), _stream()), "unpack_cache")
+            _code(out.dtype), 0, _stream()), "unpack_cache")
 
     def _paged_attention_fp4(self, q, cache, meta, out, scale, window, lse):
         """Attention over a 4-bit cache.  In bfloat16, at the head sizes its kernel takes, items of few rows (the
@@ -520,7 +520,8 @@ class HipKernels:
             scratch = torch.empty(pairs.shape[0], 2, kv_heads, page, head_dim, dtype=q.dtype, device=q.device)
             _check(_fn.get("cache_fp4", "se_fp4_unpack")(
                 _ptr(cache), _ptr(meta.block_table), meta.block_table.stride(0), _ptr(pairs), pairs.shape[0], _ptr(scratch),
-                kv_heads, page, head_dim, _code(q.dtype), _stream()), "paged_attention (unpacking 4-bit pages)")
+                kv_heads, page, head_dim, _code(q.dtype), int(work is not None and head_dim <= 256), _stream()),
+                "paged_attention (unpacking 4-bit pages)")
         if not direct:
             if q.dtype == torch.bfloat16 and head_dim <= 256:
                 self._run_attention_work(q, scratch, scratch_table, work, out, scale, window, lse, unpacked=True)
@@ -665,8 +666,8 @@ class HipKernels:
         logarithm of its sum of exponentials.  A uint8 ``cache`` holds keys and values in 4 bits (``[pages, 2, kv_heads,
         page_size, head_dim * 17 / 32]``, cache/layout.py): ``meta`` then needs its items, ``scale`` is positive, and
         the call allocates what its longer way needs: partial results, and for the portions of prompts that it reads
-        through unpacked pages a copy of those in ``q``'s type.  (There, as over the engine's own cache, a value that is
-        not a number reaches the rows of earlier tokens in its block too.)"""
+        through unpacked pages a copy of those in ``q``'s type.  A key or value that is not a number reaches the rows that
+        see it and no others; over unpacked pages in bfloat16 all dims of theirs, else the value's groups of 32."""
         tokens, heads, head_dim = q.shape
         kv_heads, page_size = cache.shape[2], cache.shape[3]
         _require(q.stride(2) == 1 and q.stride(1) == head_dim, "q heads must be dense")

@@ -61,6 +61,9 @@ def test_portions_in_unpacked_blocks(guard, monkeypatch):
         for case in C.ATTEND[11:14]:
             C.test_attention_of_many_rows_in_unpacked_blocks(hip, monkeypatch, *case)
         C.test_a_step_without_tokens(hip)
+        for which in (0, 1):
+            C.test_a_token_that_is_not_a_number_in_unpacked_pages(hip, monkeypatch, BF16, 64, 90, 20, which)
+            C.test_a_token_that_is_not_a_number_in_unpacked_pages(hip, monkeypatch, F32, 64, 20, 0, which)
         for kind in ("fp4", "own"):
             C.test_eviction_from_a_table_with_pages_given_back(hip, kind)
 

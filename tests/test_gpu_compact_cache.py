@@ -369,6 +369,34 @@ def test_a_token_that_is_not_a_number_is_seen_by_its_readers_only(hip, d, which)
     assert torch.isnan(lse[2:]).all() if which == 0 else torch.isfinite(lse).all()
 
 
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("dtype,d,new,window", [(torch.bfloat16, 128, 90, 0), (torch.bfloat16, 64, 90, 20), (torch.bfloat16, 96, 90, 0),
+                                                (torch.bfloat16, 160, 5, 0), (torch.float32, 64, 20, 0), (torch.bfloat16, 288, 5, 0)])
+def test_a_token_that_is_not_a_number_in_unpacked_pages(hip, monkeypatch, dtype, d, new, window, which):
+    """The same where attention reads unpacked pages: rows before the token, and those whose window has passed it, are as
+    if it were any other; its readers are not numbers, at least in the dims of its group."""
+    from sparseengine_amd.kernels import attention_work
+    monkeypatch.setattr(attention_work, "FP4_BLOCK_WORK", 0)
+    heads, kv, page, ctx, scale = 6, 2, 32, [130], d ** -0.5
+    bad, head, group = 130 - new + 3, 1, 1           # the step's fourth token, one kv head, dims 32 to 63
+    meta, cache, q, of = attention_case("fp4", dtype, heads, kv, d, page, ctx, [new], window)
+    place = [meta.block_table[0, bad // page].cpu().long().reshape(1), torch.tensor([bad % page])]
+    held = layout.fp4_read(cache, which, *place)
+    held[0, head, 32 * group] = float("nan")
+    layout.fp4_write(cache, which, *place, held)
+    out, lse = torch.empty(new, heads * d, dtype=dtype).to(DEV), torch.empty(new, heads).to(DEV)
+    hip.paged_attention(q.to(DEV), cache.to(DEV), meta, out, scale, window, lse=lse)
+    pos = torch.arange(130 - new, 130)
+    sees = (pos >= bad) & (pos - window < bad if window else True)
+    readers = sees[:, None] & (torch.arange(heads) // (heads // kv) == head)[None, :]
+    out, lse = out.cpu().reshape(new, heads, d), lse.cpu()
+    assert torch.isnan(out[readers][:, 32 * group:32 * group + 32]).all()
+    want, want_lse, spread, size = oracle.attention(q, of(0), of(1), ctx, [new], scale, window)      # the token as it was before
+    bound = spread * (2.0 ** -24 * (2 * (d + 8) * size + 130 + 64)[..., None] + half_step(dtype)) + half_step(dtype) * want.abs()
+    assert bool(((out.double() - want).abs() <= bound + 1e-30)[~readers].all())
+    assert bool(((lse.double() - want_lse).abs() <= 2.0 ** -24 * (2 * (d + 8) * size + 130 + 64) + 2.0 ** -22 * want_lse.abs())[~readers].all())
+
+
 # ---------------------------------------------------------------------------------------------- gathered weights
 @pytest.mark.parametrize("kind", ["fp4", "own"])
 @pytest.mark.parametrize("dtype", DTYPES)
