@@ -17,7 +17,7 @@
 // product, the running sum of them unrounded.
 //
 // Bound by reading the cache where there are keys enough, and by the latency of a wavefront's first loads else.  48:8
-// heads of 128: 4 requests of up to 131071 keys 62 us (6.7 TB/s) and 4.8 us for the merge of their ranges; 8 of up to
+// heads of 128: 4 requests of up to 131071 keys 67 us (6.1 TB/s) and 4.8 us for the merge of their ranges; 8 of up to
 // 2100 keys 9.0 + 3.7 us; one of 77 keys 6 us.
 //
 // head_dim 64, 128 or 256, page_size % 32 == 0 (a step of 32 keys lies in one page).

@@ -66,7 +66,7 @@ class DeviceAttentionWork:
 
 # A cache in 4 bits (the same heads; the kernel alone would be bound by reading at one wavefront per SIMD, and a few
 # too many, which run beside the others on some SIMDs, cost as much as twice as many everywhere).  4 requests of up to
-# 131071 keys take 70 us in at most 1024 ranges (6.9 TB/s in the kernel), 78 us in 2048, 85 us in 768; 16 x 16384 keys 44
+# 131071 keys take 70 us in at most 1024 ranges (6.1 TB/s in the kernel), 78 us in 2048, 85 us in 768; 16 x 16384 keys 44
 # against 49 us; but 64 requests x 8 heads are 512 tiles, whose ranges come in halves: 64 x 8200 keys 150 us unsplit,
 # 88 us in 2048.  A request of 77 keys takes 5.7 us whole and 7.4 in two ranges, 300 keys 9.5 us whole and 8.1 in five.
 # At head size 64 a step has half the bytes and one wavefront per SIMD is not enough (4 x 131071 keys, 32:8 heads: 50 us
