@@ -666,7 +666,8 @@ static void launch_weights_mfma(const void* q, int64_t q_stride, const void* cac
   if constexpr (ONE_TILE_FP4) {
     if (tiles <= 1) {
       // groups of a wavefront, in whole rounds of those on their way
-      const int span = window > 0 && window + most_new + 62 < longest ? window + most_new + 62 : longest;
+      const int64_t reach = static_cast<int64_t>(window) + most_new + 62;      // a window may be as long as an int holds
+      const int64_t span = window > 0 && reach < longest ? reach : longest;
       const int64_t groups = (span + 31) / 32, all = groups * kv_heads * items;
       int per_wave = static_cast<int>((all + ONE_TILE_WAVES - 1) / ONE_TILE_WAVES);
       per_wave = (per_wave + ONE_TILE_DEPTH - 1) / ONE_TILE_DEPTH * ONE_TILE_DEPTH;

@@ -1,0 +1,22 @@
+"""The bodies of tests/test_gpu_compact_edges.py on the CPU: the kernel sources built for the host, every tensor argument
+next to an inaccessible page."""
+import pytest
+import torch
+
+import tests.test_gpu_compact_edges as G
+from tests import backends
+from tests.test_emu_compact_cache import Emulated
+
+pytestmark = pytest.mark.skipif(not backends.EmulatedBackend().available(), reason="no host compiler for the emulated kernels")
+
+
+@pytest.fixture(params=["after", "before"])
+def guard(request):
+    return request.param
+
+
+@pytest.mark.parametrize("case", G.WIDE_WINDOWS)
+def test_weights_under_a_window_as_long_as_everything(guard, case):
+    with Emulated(guard=guard) as hip:
+        for kind in ("fp4", "own"):
+            G.test_weights_under_a_window_as_long_as_everything(hip, kind, case)
