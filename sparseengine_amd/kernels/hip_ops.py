@@ -68,6 +68,12 @@ def _same_device(*tensors):
         raise ValueError("the tensors of a call must be on the current device")
 
 
+def _window(window) -> int:
+    """An attention window as the kernels take it, in 32 bits: 0 for none."""
+    _require(not window or window > 0, "an attention window must not be below 0 (0: none)")
+    return min(int(window or 0), 0x7fffffff)
+
+
 def _i32(t: torch.Tensor, name: str):
     _require(t.dtype == torch.int32 and t.is_contiguous(), f"{name} must be contiguous int32")
 
@@ -558,6 +564,7 @@ class HipKernels:
         are left as they are.  No two items share a page."""
         tokens, heads, head_dim = q.shape
         fp4 = cache.dtype == torch.uint8
+        window = _window(window)
         _require(q.stride(2) == 1 and q.stride(1) == head_dim, "q heads must be dense")
         if fp4:
             self._fp4_cache(cache, head_dim)
@@ -589,7 +596,7 @@ class HipKernels:
         _check(_fn.get("attention_weights", "se_attention_weights")(
             _ptr(q), q.stride(0), _ptr(cache), self._CACHE_KINDS[cache.dtype], _ptr(meta.block_table),
             meta.block_table.stride(0), _ptr(item_meta), items, longest, most_new, _ptr(lse), _ptr(previous), _ptr(out), heads, kv_heads,
-            head_dim, page, float(scale), int(window or 0), _code(q.dtype), _ptr(workspace), _stream()), "attention_weights")
+            head_dim, page, float(scale), window, _code(q.dtype), _ptr(workspace), _stream()), "attention_weights")
 
     @staticmethod
     def _check_items(meta, tokens: int, page: int, what: str):
@@ -664,7 +671,7 @@ class HipKernels:
         optionally prepared work lists (``work``);
         ``out``: ``[T, heads * head_dim]``; ``lse``: None, or float32 ``[T, heads]`` that receives every row's
         logarithm of its sum of exponentials.  A uint8 ``cache`` holds keys and values in 4 bits (``[pages, 2, kv_heads,
-        page_size, head_dim * 17 / 32]``, cache/layout.py): ``meta`` then needs its items, ``scale`` is positive, and
+        page_size, head_dim * 17 / 32]``, cache/layout.py): ``meta`` then needs its items, ``scale`` is positive, ``window`` not negative, and
         the call allocates what its longer way needs: partial results, and for the portions of prompts that it reads
         through unpacked pages a copy of those in ``q``'s type.  A key or value that is not a number reaches the rows that
         see it and no others; over unpacked pages in bfloat16 all dims of theirs, else the value's groups of 32."""
@@ -676,7 +683,7 @@ class HipKernels:
             # a step of few rows per item with its work list prepared, in one expression; every other call, and one that
             # fails a check, takes the long way, which names what is wrong
             work, table = meta.work.get((heads // kv_heads if kv_heads else 0, window, "fp4")), meta.block_table
-            if (work is not None and not work.num_block_units and heads % kv_heads == 0 and scale > 0
+            if (work is not None and not work.num_block_units and 0 <= window <= 0x7fffffff and heads % kv_heads == 0 and scale > 0
                     and q.dtype == torch.bfloat16 and head_dim in FP4_HEAD_DIMS and q.stride(0) % 8 == 0
                     and cache.dim() == 5 and cache.shape[1] == 2 and cache.shape[4] * 32 == head_dim * 17 and page_size % 32 == 0
                     and cache.is_contiguous()
@@ -703,6 +710,7 @@ class HipKernels:
             raise KernelShapeError(f"attention: page_size {page_size} must be a multiple of 8")
         window = int(window or 0)
         if fp4:
+            window = _window(window)
             _same_device(q, cache, out, lse, meta.block_table)
             if q.stride(0) % 8 or out.stride(0) % 8 or q.data_ptr() % 16 or out.data_ptr() % 16:
                 raise KernelShapeError("attention over a 4-bit cache: rows of q and out have to begin on multiples of 16 bytes")

@@ -20,3 +20,9 @@ def test_weights_under_a_window_as_long_as_everything(guard, case):
     with Emulated(guard=guard) as hip:
         for kind in ("fp4", "own"):
             G.test_weights_under_a_window_as_long_as_everything(hip, kind, case)
+
+
+def test_windows_that_32_bits_do_not_hold():
+    with Emulated() as hip:
+        for kind in ("fp4", "own"):
+            G.test_windows_that_32_bits_do_not_hold(hip, kind)

@@ -35,3 +35,22 @@ WIDE_WINDOWS = [  # heads, kv_heads, head_dim, page, contexts, new tokens, windo
 @pytest.mark.parametrize("case", WIDE_WINDOWS)
 def test_weights_under_a_window_as_long_as_everything(hip, kind, case):
     C.test_weights_of_the_cached_keys(hip, BF16, kind, *case)
+
+
+@pytest.mark.parametrize("kind", ["fp4", "own"])
+def test_windows_that_32_bits_do_not_hold(hip, kind):
+    """A window of more tokens than an int counts is none; one below 0 is refused."""
+    case = (6, 1, 64, 32, [70, 5], [1, 2])
+    for window in (2 ** 31, 2 ** 32 + 5):
+        if kind == "fp4":
+            C.test_attention_in_4_bits(hip, BF16, *case, window)
+        C.test_weights_of_the_cached_keys(hip, BF16, kind, *case, window)
+        C.test_weights_of_the_cached_keys(hip, F32, kind, *case, window)
+    meta, cache, q, _ = C.attention_case(kind, BF16, *case, 0)
+    out, lse, weights = torch.empty(3, 6 * 64, dtype=BF16), torch.zeros(3, 6), torch.zeros(cache.shape[0], 1, 32)
+    cache, q, out, lse, weights = (t.to(C.DEV) for t in (cache, q, out, lse, weights))
+    with pytest.raises(ValueError, match="window"):
+        hip.attention_weights(q, cache, meta, lse, weights, 0.125, -1)
+    if kind == "fp4":
+        with pytest.raises(ValueError, match="window"):
+            hip.paged_attention(q, cache, meta, out, 0.125, -1)
