@@ -716,6 +716,7 @@ extern "C" int se_attention_weights(const void* q, int64_t q_stride, const void*
   if (kind == SE_CACHE_FP4 && (head_dim % 32 || page_size % 32)) return SE_ERR_SHAPE;
   if (kind != SE_CACHE_FP4 && kind != (dtype == SE_F32 ? SE_CACHE_F32 : SE_CACHE_BF16)) return SE_ERR_SHAPE;
   if (kv_heads > 65535 || items > 65535) return SE_ERR_SHAPE;
+  if (!(scale > 0.f)) return SE_ERR_SHAPE;      // masked scores are -inf before it is applied
   const int64_t most_rows = static_cast<int64_t>(most_new) * (heads / kv_heads);
   if (weights_on_matrix_cores(head_dim, most_rows, dtype)) {
     const int splits = se_attention_weights_splits(items, longest, most_new, heads, kv_heads, head_dim, dtype);

@@ -558,7 +558,7 @@ class HipKernels:
         head's query heads and the step's tokens): ``out[key] = previous[key] + sum exp(scale q . k - lse)``.
 
         ``q``, ``cache``, ``meta``, ``scale`` and ``window`` as in ``paged_attention``, whose ``lse [T, heads]`` (float32)
-        goes in here; ``meta`` needs its items.  ``out`` and ``previous``: float32 ``[pages, kv_heads, page_size]`` in
+        goes in here; ``meta`` needs its items, ``scale`` is positive, ``window`` not negative.  ``out`` and ``previous``: float32 ``[pages, kv_heads, page_size]`` in
         the cache's pages; they may be the same tensor.  ``previous`` counts for the keys that are older than the
         step (None: nothing for them either); the step's own keys begin with 0.  Keys that no row can see (a window)
         are left as they are.  No two items share a page."""
@@ -583,6 +583,7 @@ class HipKernels:
                      f"attention weights: {name} must be contiguous float32 [pages, kv_heads, page_size]")
         _require(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (tokens, heads),
                  "attention weights: lse must be contiguous float32 [tokens, heads]")
+        _require(scale > 0, "attention weights: scale must be positive")
         _require(meta.block_table.dtype == torch.int32 and meta.block_table.dim() == 2 and meta.block_table.stride(1) == 1,
                  "block_table layout")
         if tokens == 0:

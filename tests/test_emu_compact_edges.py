@@ -26,3 +26,10 @@ def test_windows_that_32_bits_do_not_hold():
     with Emulated() as hip:
         for kind in ("fp4", "own"):
             G.test_windows_that_32_bits_do_not_hold(hip, kind)
+
+
+def test_weights_refuse_a_scale_that_is_not_positive():
+    with Emulated() as hip:
+        for kind in ("fp4", "own"):
+            for dtype in (G.BF16, G.F32):
+                G.test_weights_refuse_a_scale_that_is_not_positive(hip, kind, dtype)

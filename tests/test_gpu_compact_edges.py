@@ -54,3 +54,15 @@ def test_windows_that_32_bits_do_not_hold(hip, kind):
     if kind == "fp4":
         with pytest.raises(ValueError, match="window"):
             hip.paged_attention(q, cache, meta, out, 0.125, -1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kind", ["fp4", "own"])
+def test_weights_refuse_a_scale_that_is_not_positive(hip, kind, dtype):
+    """Masked scores are the lowest there are before the scale is applied: one below 0 would make them the largest."""
+    meta, cache, q, _ = C.attention_case(kind, dtype, 6, 1, 64, 32, [70], [5], 0)
+    weights = torch.full((cache.shape[0], 1, 32), 9.0).to(C.DEV)
+    for scale in (0.0, -0.125, float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            hip.attention_weights(q.to(C.DEV), cache.to(C.DEV), meta, torch.zeros(5, 6).to(C.DEV), weights, scale)
+    assert (weights == 9).all()
