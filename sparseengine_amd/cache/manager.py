@@ -305,7 +305,7 @@ class CacheManager:
     # ------------------------------------------------------------------ letting tokens go
     def begin_eviction(self, rows, keep: int) -> dict[int, np.ndarray]:
         """Fresh pages for ``keep`` tokens of every listed row: group index -> int32 ``[rows, ceil(keep / page_size)]``.
-        They belong to the rows, beside their old ones, until ``finish_eviction``; all or nothing."""
+        They belong to the rows, beside their old ones, until ``finish_eviction`` or ``abort_eviction``; all or nothing."""
         for group in self.groups:
             if group.window is not None:
                 raise ValueError("a windowed cache group gives its tokens back by itself")
@@ -316,6 +316,12 @@ class CacheManager:
                 raise ValueError(f"row {row} holds {self.row_len[row]} tokens: it cannot keep {keep}")
         return {group.index: np.asarray([group.pool.allocate(-(-keep // group.page_size), row) for row in rows], dtype=np.int32)
                 for group in self.groups}
+
+    def abort_eviction(self, rows, tables: dict[int, np.ndarray]) -> None:
+        """The tokens could not be moved: the fresh pages of ``tables`` return to the pool, the rows stay as they were."""
+        for group in self.groups:
+            for row, pages in zip(rows, tables[group.index]):
+                group.pool.release(pages.tolist(), row)
 
     def finish_eviction(self, rows, keep: int, tables: dict[int, np.ndarray]) -> None:
         """The rows' tokens have been moved to the pages of ``tables``: their old pages return to the pool."""

@@ -83,14 +83,18 @@ class AccumulatedWeightMethod(MethodRuntime):
         lengths = cache.row_len[rows].astype(np.int32)
         longest = int(lengths.max())
         tables = cache.begin_eviction(rows, keep)
-        on_device = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(fb.device)
-        lengths_there = on_device(lengths)
-        for group in cache.groups:
-            old = on_device(group.table[rows, :-(-longest // group.page_size)])
-            new = on_device(tables[group.index])
-            kept = fb.buffer("evict.kept", (len(rows), group.request.kv_heads, keep), torch.int32)
-            for position, layer in group.layers.items():
-                fb.kernels.evict_tokens(layer, self.weights[position], old, lengths_there, new, keep, self.recent, kept,
-                                        longest=longest)
+        try:
+            on_device = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(fb.device)
+            lengths_there = on_device(lengths)
+            for group in cache.groups:
+                old = on_device(group.table[rows, :-(-longest // group.page_size)])
+                new = on_device(tables[group.index])
+                kept = fb.buffer("evict.kept", (len(rows), group.request.kv_heads, keep), torch.int32)
+                for position, layer in group.layers.items():
+                    fb.kernels.evict_tokens(layer, self.weights[position], old, lengths_there, new, keep, self.recent, kept,
+                                            longest=longest)
+        except Exception:      # the old pages are as they were
+            cache.abort_eviction(rows, tables)
+            raise
         cache.finish_eviction(rows, keep, tables)
         self.evictions += len(rows)

@@ -1,0 +1,58 @@
+"""The host's account under eviction and with a cache in 4 bits: pages, reserves, memory, work lists (no kernel runs)."""
+import numpy as np
+import pytest
+import torch
+
+from sparseengine_amd import LLM, SamplingParams
+from tests.helpers import make_folder, random_tokens
+from tests.twin_kernels import TwinKernels
+
+
+class Twins(TwinKernels):
+    """The twins of the dense path; gathered weights and eviction do nothing."""
+
+    def paged_attention(self, q, cache, meta, out, scale, window=0, lse=None):
+        super().paged_attention(q, cache, meta, out, scale, window)
+
+    def attention_weights(self, *args, **kwargs):
+        pass
+
+    def evict_tokens(self, *args, **kwargs):
+        pass
+
+
+def evicting(tmp_path, kernels=None, **kwargs):
+    return LLM(make_folder(tmp_path, "A_loud"), _kernels=kernels or Twins(), _device="cpu", **{**dict(
+        dtype="float32", kv_page_size=16, num_kvcache_slots=192, max_num_seqs_in_batch=4, max_num_batched_tokens=32,
+        engine_prefill_chunk_size=16, sparse_method="accumulated_weight", eviction_budget=33, validate_runtime_invariants=True), **kwargs})
+
+
+def greedy(n):
+    return SamplingParams(temperature=0.0, max_tokens=n, ignore_eos=True)
+
+
+@pytest.mark.parametrize("fails_at", [1, 2, 3])
+def test_a_cut_that_fails_gives_its_pages_back(tmp_path, fails_at):
+    """An error while tokens are moved: the step is undone, the fresh pages are free again, and what runs next finds the
+    whole cache."""
+    class Failing(Twins):
+        calls = 0
+
+        def evict_tokens(self, *args, **kwargs):
+            Failing.calls += 1
+            if Failing.calls == fails_at:
+                raise RuntimeError("no room to move the tokens in")
+
+    llm = evicting(tmp_path, Failing())
+    prompts = [random_tokens(n, 512, n) for n in (90, 61)]
+    for p in prompts:
+        llm.add_request(p, greedy(20))
+    with pytest.raises(RuntimeError, match="no room"):
+        while not llm.is_finished():
+            llm.step()
+    cache = llm.runner.cache
+    cache.check_invariants()
+    while not llm.is_finished():
+        llm.step()
+    cache.check_invariants()
+    assert Failing.calls > fails_at and all(g.pool.free_count == g.pool.num_pages for g in cache.groups)
