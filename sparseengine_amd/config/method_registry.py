@@ -34,6 +34,8 @@ class MethodRuntime:
     ``tokens_taken(length, n)``    how many more tokens of cache a request that holds ``length`` takes at most
                                    while ``n`` are added to it, in steps' portions (the dense method: n);
     ``reserved_pages()``           {group index: pages} that no request may take;
+    ``reserved_tokens(page, longest)`` before there is a cache: tokens of cache that hold those pages, for pages of at most
+                                   ``page`` tokens and requests of at most ``longest``;
     ``kernel_libraries``           the kernel libraries it calls;
     ``configure(config)``          once, before the runner is built, with the runtime configuration;
     ``bytes_per_token(request)``   device memory the method keeps per cached token and position beside the cache;
@@ -63,6 +65,9 @@ class MethodRuntime:
 
     def reserved_pages(self) -> dict[int, int]:
         return {}
+
+    def reserved_tokens(self, page: int, longest: int) -> int:
+        return 0
 
     def bytes_per_token(self, request) -> int:
         return 0

@@ -61,6 +61,9 @@ class AccumulatedWeightMethod(MethodRuntime):
             return {}
         return {g.index: -(-self.budget // g.page_size) for g in self.cache.groups}
 
+    def reserved_tokens(self, page: int, longest: int) -> int:
+        return self.budget + page - 1 if self.budget + page <= longest else 0
+
     def tokens_taken(self, length: int, new_tokens: int) -> int:
         # less than the limit between two steps, and what one step adds
         return max(min(new_tokens, max(1, self.portion)), min(new_tokens, self._limit() - 1 + max(1, self.portion) - length))

@@ -127,19 +127,20 @@ class ModelRunner:
 
     def derive_cache_tokens(self, requests, max_num_seqs: int, utilization: float) -> int:
         """Tokens of cache that fit the memory left after the weights: ``utilization`` of the card
-        minus what is in use, capped by what ``max_num_seqs`` requests of full length could hold."""
+        minus what is in use, capped by what ``max_num_seqs`` requests of full length could hold beside what the method
+        reserves."""
         from ..parts.base import PagedKVRequest
         per_token = sum(bytes_per_token(r, self.kv_dtype) + self.method.bytes_per_token(r) for r in requests.values()
                         if isinstance(r, PagedKVRequest))
-        cap = max_num_seqs * self.max_model_len
+        largest_page = max([self.kv_page_size] + [r.page_size or 0 for r in requests.values() if isinstance(r, PagedKVRequest)])
+        cap = max_num_seqs * self.max_model_len + self.method.reserved_tokens(largest_page, self.max_model_len)
         if per_token == 0 or self.device.type != "cuda":
             return cap
         free, total = torch.cuda.mem_get_info(self.device)
         usable = free - int((1.0 - utilization) * total) - (2 << 30)      # 2 GiB kept for step buffers
         if self.kv_dtype != self.dtype:      # and what a step's portions of two longest prompts unpack for a layer
             usable -= 2 * self.max_model_len * max(bytes_per_token(r, self.dtype) for r in requests.values() if isinstance(r, PagedKVRequest))
-        if usable <= per_token * max([self.kv_page_size] + [r.page_size or 0 for r in requests.values()
-                                                            if isinstance(r, PagedKVRequest)]):
+        if usable <= per_token * largest_page:
             raise RuntimeError("no GPU memory is left for the cache after the weights")
         return min(cap, usable // per_token)
 

@@ -56,3 +56,16 @@ def test_a_cut_that_fails_gives_its_pages_back(tmp_path, fails_at):
         llm.step()
     cache.check_invariants()
     assert Failing.calls > fails_at and all(g.pool.free_count == g.pool.num_pages for g in cache.groups)
+
+
+@pytest.mark.parametrize("seqs", [1, 2])
+def test_a_cache_of_the_engines_own_size_holds_full_requests_beside_the_reserve(tmp_path, seqs):
+    """Without a number of cache slots the cache has room for so many requests of full length: the pages that eviction
+    reserves come on top, and a request as long as the model allows is served."""
+    most = 160
+    llm = evicting(tmp_path, num_kvcache_slots=None, max_num_seqs_in_gpu=seqs, max_num_seqs_in_batch=seqs, max_model_len=most,
+                   max_num_batched_tokens=most, engine_prefill_chunk_size=most, eviction_budget=100)
+    prompts = [random_tokens(most - 8, 512, i) for i in range(seqs)]
+    out = llm.generate(prompts, greedy(8), use_tqdm=False)
+    assert [len(o["token_ids"]) for o in out] == [8] * seqs and llm.method.evictions >= seqs
+    llm.runner.cache.check_invariants()
