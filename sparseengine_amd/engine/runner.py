@@ -181,8 +181,8 @@ class ModelRunner:
         self.cache.free(request_id)
 
     def can_step(self, entries) -> bool:
-        """Whether the cache has room for these (request_id, new token count) pairs; requests
-        not yet admitted are counted with an empty row."""
+        """Whether the cache has room for these (request_id, new token count) pairs beside the pages that the method
+        reserves; requests not yet admitted are counted with an empty row."""
         need = {g.index: 0 for g in self.cache.groups}
         new_rows = 0
         for request_id, n in entries:
@@ -196,8 +196,8 @@ class ModelRunner:
                     need[gi] += pages
             for gi, pages in self.method.extra_pages(row, n).items():
                 need[gi] += pages
-        free = self.cache.free_pages()
-        return new_rows <= self.cache.num_free_rows and all(need[g] <= free[g] for g in need)
+        free, reserved = self.cache.free_pages(), self.method.reserved_pages()
+        return new_rows <= self.cache.num_free_rows and all(need[g] <= free[g] - reserved.get(g, 0) for g in need)
 
     # ------------------------------------------------------------------ the step
     @torch.no_grad()

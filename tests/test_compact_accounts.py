@@ -69,3 +69,26 @@ def test_a_cache_of_the_engines_own_size_holds_full_requests_beside_the_reserve(
     out = llm.generate(prompts, greedy(8), use_tqdm=False)
     assert [len(o["token_ids"]) for o in out] == [8] * seqs and llm.method.evictions >= seqs
     llm.runner.cache.check_invariants()
+
+
+def test_can_step_leaves_the_reserved_pages_alone(tmp_path):
+    """A caller that drives the runner by ``can_step``: it says no before a step would take the pages that a cut needs, and
+    every request that it lets run is cut when its time comes."""
+    # a request reaches its cut in 4 pages (33 + 16 tokens and a step's): two do, beside 3 pages in reserve
+    runner = evicting(tmp_path, num_kvcache_slots=16 * 13).runner
+    from sparseengine_amd.engine.runner import StepEntry
+    reserved = runner.method.reserved_pages()[0]
+    group, fed = runner.cache.groups[0], {}
+    for turn in range(300):
+        entries = [(name, 5) for name in ("a", "b", "c")]
+        entries = [entries[turn % 3]]
+        if runner.can_step(entries):
+            name, n = entries[0]
+            runner.step([StepEntry(name, random_tokens(n, 512, turn))])
+            fed[name] = fed.get(name, 0) + n
+            assert group.pool.free_count >= reserved and runner.cache.row_len[runner.cache.row_of(name)] < runner.method._limit()
+        if max(fed.values()) > 150:
+            break
+    assert runner.method.evictions > 0
+    assert not runner.can_step([("d", (group.pool.free_count - reserved) * 16 + 1)])
+    assert runner.can_step([("d", (group.pool.free_count - reserved) * 16)])
