@@ -14,6 +14,7 @@ import torch
 
 from ..cache.manager import CacheManager, bytes_per_token
 from ..config.registry import Architecture, read_config_json, resolve_architecture
+from ..kernels.attention_work import FP4_HEAD_DIMS
 from ..weights import loader as weight_loader
 from ..weights import random_weights
 from .batch import BatchBuilder, StepItem
@@ -138,8 +139,14 @@ class ModelRunner:
             return cap
         free, total = torch.cuda.mem_get_info(self.device)
         usable = free - int((1.0 - utilization) * total) - (2 << 30)      # 2 GiB kept for step buffers
-        if self.kv_dtype != self.dtype:      # and what a step's portions of two longest prompts unpack for a layer
-            usable -= 2 * self.max_model_len * max(bytes_per_token(r, self.dtype) for r in requests.values() if isinstance(r, PagedKVRequest))
+        if self.kv_dtype != self.dtype:      # what attention over 4 bits unpacks, one layer at a time
+            paged = [r for r in requests.values() if isinstance(r, PagedKVRequest)]
+            direct = [r for r in paged if self.dtype == torch.bfloat16 and r.head_dim in FP4_HEAD_DIMS]
+            whole = [bytes_per_token(r, self.dtype) for r in paged if r not in direct]
+            if whole:        # sizes without a kernel that reads 4 bits: all that the step's requests have cached
+                per_token += max(whole)
+            if direct:       # the portions of two longest prompts
+                usable -= 2 * self.max_model_len * max(bytes_per_token(r, self.dtype) for r in direct)
         if usable <= per_token * largest_page:
             raise RuntimeError("no GPU memory is left for the cache after the weights")
         return min(cap, usable // per_token)

@@ -1,9 +1,15 @@
 """The host's account under eviction and with a cache in 4 bits: pages, reserves, memory, work lists (no kernel runs)."""
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 import torch
 
 from sparseengine_amd import LLM, SamplingParams
+from sparseengine_amd.cache.manager import bytes_per_token
+from sparseengine_amd.config.method_registry import PassThroughMethod
+from sparseengine_amd.engine.runner import ModelRunner
+from sparseengine_amd.parts.base import PagedKVRequest
 from tests.helpers import make_folder, random_tokens
 from tests.twin_kernels import TwinKernels
 
@@ -92,3 +98,23 @@ def test_can_step_leaves_the_reserved_pages_alone(tmp_path):
     assert runner.method.evictions > 0
     assert not runner.can_step([("d", (group.pool.free_count - reserved) * 16 + 1)])
     assert runner.can_step([("d", (group.pool.free_count - reserved) * 16)])
+
+
+@pytest.mark.parametrize("layers", [1, 2, 32])
+@pytest.mark.parametrize("dtype,head_dim,direct", [(torch.bfloat16, 96, False), (torch.float32, 128, False),
+                                                   (torch.bfloat16, 288, False), (torch.bfloat16, 128, True)])
+def test_memory_kept_for_unpacked_pages(monkeypatch, dtype, head_dim, direct, layers):
+    """The cache that the engine chooses leaves room for what attention unpacks of one layer: where a head size or type has
+    no kernel that reads 4 bits, every token that the cache holds (a full decode step reads them all)."""
+    free, total = 60 << 30, 64 << 30
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device=None: (free, total))
+    requests = {i: PagedKVRequest(4, head_dim, None, None) for i in range(layers)}
+    runner = SimpleNamespace(kv_dtype=torch.uint8, dtype=dtype, device=torch.device("cuda"), max_model_len=4096, kv_page_size=64,
+                             method=PassThroughMethod())
+    tokens = ModelRunner.derive_cache_tokens(runner, requests, 1 << 20, 0.9)
+    usable = free - int(0.1 * total) - (2 << 30)
+    held = layers * bytes_per_token(requests[0], torch.uint8)
+    unpacked = bytes_per_token(requests[0], dtype)
+    at_once = 2 * 4096 if direct else tokens
+    assert tokens * held + at_once * unpacked <= usable          # and no more is left unused than a token of each
+    assert (tokens + 1) * held + (at_once + (not direct)) * unpacked > usable
