@@ -20,7 +20,7 @@ constexpr int BLOCK_UNIT_FIELDS = 12;
 
 struct Rules {  // order of the `rules` argument
   int64_t target_waves, min_split_keys, max_splits, tiles_per_block, tiled_max_head_dim, target_blocks,
-      min_block_keys, prefix_per_portion, block_tiles;      // block_tiles: what an item needs to go in blocks
+      min_block_keys, prefix_per_portion;
 };
 
 // per item: in_blocks, rows (tiles or blocks), splits, chunk, first_key, base
@@ -44,12 +44,13 @@ int64_t keys_per_unit(const std::vector<int64_t>& units_per_item, const std::vec
 
 extern "C" {
 
-// plan: int64 [items, PLAN_FIELDS]; counts: int64 [4] = units, tasks, block units, partial slots
+// block_tiles: int64 [items], the tiles that an item needs to go in blocks; plan: int64 [items, PLAN_FIELDS];
+// counts: int64 [4] = units, tasks, block units, partial slots
 int se_attention_work_plan(const int64_t* q_len, const int64_t* ctx_len, int items, int group,
-                           int kv_heads, int window, int head_dim, const int64_t* rules_in,
+                           int kv_heads, int window, int head_dim, const int64_t* block_tiles, const int64_t* rules_in,
                            int64_t* plan, int64_t* counts) {
   if (items < 0 || group <= 0 || kv_heads <= 0) return -1;
-  Rules r{rules_in[0], rules_in[1], rules_in[2], rules_in[3], rules_in[4], rules_in[5], rules_in[6], rules_in[7], rules_in[8]};
+  Rules r{rules_in[0], rules_in[1], rules_in[2], rules_in[3], rules_in[4], rules_in[5], rules_in[6], rules_in[7]};
   const bool blocks_allowed = head_dim > 0 && head_dim % 32 == 0 && head_dim <= r.tiled_max_head_dim;
   std::vector<int64_t> tiles(items), reach(items), nblocks(items), alone(items), cut_blocks(items);
   int64_t whole = 0;      // blocks of items that are never cut into key ranges
@@ -57,7 +58,7 @@ int se_attention_work_plan(const int64_t* q_len, const int64_t* ctx_len, int ite
     if (q_len[i] < 1 || q_len[i] > ctx_len[i]) return -2;   // an item's new tokens are part of its context
     tiles[i] = (q_len[i] * group + 15) / 16;
     reach[i] = window ? std::min<int64_t>(ctx_len[i], window + q_len[i]) : ctx_len[i];
-    const bool in_blocks = blocks_allowed && tiles[i] >= r.block_tiles;
+    const bool in_blocks = blocks_allowed && tiles[i] >= block_tiles[i];
     plan[i * PLAN_FIELDS + 0] = in_blocks;
     nblocks[i] = in_blocks ? ceil_div(tiles[i], r.tiles_per_block) : 0;
     alone[i] = in_blocks ? 0 : tiles[i];

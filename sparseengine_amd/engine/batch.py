@@ -131,12 +131,14 @@ class BatchBuilder:
     """Turns step items into a ``ForwardBatch``: cache reservation + one packed host-to-device copy."""
 
     def __init__(self, kernels, cache: CacheManager, dtype, device, vocab_size: int,
-                 attention_shapes: dict | None = None):
+                 attention_shapes: dict | None = None, most_unpacked: int | None = None):
         """``attention_shapes``: cache group index -> set of (query heads per kv head, window) whose
-        attention work lists are to be prepared with every batch."""
+        attention work lists are to be prepared with every batch.  ``most_unpacked``: the tokens of a 4-bit cache that a
+        step's prompt portions may unpack at a time (None: no limit)."""
         self.kernels, self.cache, self.dtype, self.device = kernels, cache, dtype, torch.device(device)
         self.vocab_size = vocab_size
         self.attention_shapes = attention_shapes or {}
+        self.most_unpacked = most_unpacked
         self.scratch = StepScratch()
         self._host = None
         self._dev = None
@@ -219,12 +221,16 @@ class BatchBuilder:
                 head_dim = group.request.head_dim
                 direct = fp4 and self.dtype == torch.bfloat16 and head_dim in FP4_HEAD_DIMS
                 for ratio, window in sorted(self.attention_shapes.get(group.index, ())):
-                    build = build_fp4_attention_work if direct else build_attention_work
-                    work = build(q_len, ctx_len, ratio, group.request.kv_heads, window, head_dim=head_dim)
+                    if direct:
+                        work = build_fp4_attention_work(q_len, ctx_len, ratio, group.request.kv_heads, window, head_dim,
+                                                        group.page_size, self.most_unpacked)
+                    else:
+                        work = build_attention_work(q_len, ctx_len, ratio, group.request.kv_heads, window, head_dim=head_dim)
                     works.append((group.index, (ratio, window, "fp4") if direct else (ratio, window), work, len(parts)))
                     parts += [work.units.reshape(-1), work.tasks.reshape(-1), work.block_units.reshape(-1)]
                     if fp4 and (not direct or len(work.block_units)):
-                        pairs, table = fp4_unpack_list(q_len, ctx_len, ratio, head_dim, group.page_size, window, direct)
+                        pairs, table = fp4_unpack_list(q_len, ctx_len, ratio, head_dim, group.page_size, window, direct,
+                                                       self.most_unpacked)
                         lists.append((group.index, ("unpack", ratio, head_dim, group.page_size, window, direct), pairs, table, len(parts)))
                         parts += [pairs.reshape(-1), table.reshape(-1)]
         # every part starts on a 16-byte boundary: kernels read records of four ints at once

@@ -121,8 +121,10 @@ class ModelRunner:
                 key = getattr(self.model.layers[self.spec.schedule[position].layer].mixer, "work_key", None)
                 if key is not None:
                     shapes.setdefault(self.cache.group_of_position[position], set()).add(key())
+        # a step's prompt portions unpack what two longest prompts hold, which is what derive_cache_tokens keeps memory
+        # for; those beyond are read in 4 bits
         self.builder = BatchBuilder(kernels, self.cache, self.dtype, self.device, self.spec.vocab_size,
-                                    attention_shapes=shapes)
+                                    attention_shapes=shapes, most_unpacked=2 * self.max_model_len)
         method.bind(self.cache)
         self.validate_runtime_invariants = bool(validate_runtime_invariants)
 

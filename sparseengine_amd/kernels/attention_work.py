@@ -96,7 +96,7 @@ def _native_library():
         lib = library.load("host_work")
         i64p, i32p = ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int32)
         lib.se_attention_work_plan.argtypes = [i64p, i64p, ctypes.c_int, ctypes.c_int, ctypes.c_int,
-                                               ctypes.c_int, ctypes.c_int, i64p, i64p, i64p]
+                                               ctypes.c_int, ctypes.c_int, i64p, i64p, i64p, i64p]
         lib.se_attention_work_fill.argtypes = [i64p, i64p, ctypes.c_int, ctypes.c_int, ctypes.c_int, i64p,
                                                i64p, i32p, i32p, i32p]
         _native = lib
@@ -108,20 +108,21 @@ _BAD_LENGTHS = "attention work: every item needs at least one new token and no m
 
 def build_attention_work(q_len, ctx_len, group: int, kv_heads: int, window: int = 0,
                          target_waves: int = TARGET_WAVES, head_dim: int = 0,
-                         min_split_keys: int = MIN_SPLIT_KEYS, block_tiles: int = TILES_PER_BLOCK // 2) -> AttentionWork:
+                         min_split_keys: int = MIN_SPLIT_KEYS, block_tiles=TILES_PER_BLOCK // 2) -> AttentionWork:
     """The work lists of one step, from the compiled builder; ``build_attention_work_numpy`` states
     the rules and gives the same lists (the tests compare the two), about twenty times slower."""
     lib = _native_library()
     q = np.ascontiguousarray(q_len, dtype=np.int64)
     c = np.ascontiguousarray(ctx_len, dtype=np.int64)
     rules = np.asarray([target_waves, min_split_keys, MAX_SPLITS, TILES_PER_BLOCK, TILED_MAX_HEAD_DIM,
-                        TARGET_BLOCKS, MIN_BLOCK_KEYS, PREFIX_PER_PORTION, block_tiles], dtype=np.int64)
+                        TARGET_BLOCKS, MIN_BLOCK_KEYS, PREFIX_PER_PORTION], dtype=np.int64)
+    needed = np.full(q.size, block_tiles, dtype=np.int64)      # a number for all items, or one for each
     plan = np.empty((q.size, 6), dtype=np.int64)
     counts = np.empty(4, dtype=np.int64)
     i64p, i32p = ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int32)
     as64 = lambda a: a.ctypes.data_as(i64p)
     status = lib.se_attention_work_plan(as64(q), as64(c), q.size, group, kv_heads, int(window or 0), int(head_dim or 0),
-                                        as64(rules), as64(plan), as64(counts))
+                                        as64(needed), as64(rules), as64(plan), as64(counts))
     if status == -2:
         raise ValueError(_BAD_LENGTHS)
     if status != 0:
@@ -134,11 +135,12 @@ def build_attention_work(q_len, ctx_len, group: int, kv_heads: int, window: int 
     return AttentionWork(units, tasks, int(counts[3]), blocks)
 
 
-def build_fp4_attention_work(q_len, ctx_len, group: int, kv_heads: int, window: int = 0, head_dim: int = 0) -> AttentionWork:
+def build_fp4_attention_work(q_len, ctx_len, group: int, kv_heads: int, window: int = 0, head_dim: int = 0, page: int = 1,
+                             most_unpacked: int | None = None) -> AttentionWork:
     """The work lists of a step over a cache in 4 bits: ranges that together are no more than fill the chip once (an
     item's last range is a partial one, so one is taken off the number wanted for each tile)."""
     q = np.asarray(q_len, dtype=np.int64)
-    block_tiles = fp4_block_tiles(q, ctx_len, group, window)
+    block_tiles = fp4_block_tiles(q, ctx_len, group, window, page, most_unpacked)
     tiles = int(((q * group + 15) // 16)[~items_in_blocks(q, group, head_dim, block_tiles)].sum()) * kv_heads
     wanted = FP4_WAVES if head_dim >= 128 and 4 * tiles <= FP4_WAVES else FP4_MANY_WAVES
     if q.size and int(np.max(ctx_len)) <= FP4_WHOLE_KEYS:
@@ -147,27 +149,48 @@ def build_fp4_attention_work(q_len, ctx_len, group: int, kv_heads: int, window: 
                                 block_tiles)
 
 
-def fp4_block_tiles(q_len, ctx_len, group: int, window: int) -> int:
-    """The tiles an item needs to go in blocks in a step over a cache in 4 bits."""
+def fp4_block_tiles(q_len, ctx_len, group: int, window: int, page: int = 1, most_unpacked: int | None = None):
+    """The tiles an item needs to go in blocks in a step over a cache in 4 bits: a number, or one for each item where not
+    all that have enough may.  ``most_unpacked``: the tokens that the step may unpack, in whole pages of ``page`` (None: no
+    limit); those whose rows read the most keys come first, the others stay with the kernel that reads 4 bits."""
     q, c = np.asarray(q_len, dtype=np.int64), np.asarray(ctx_len, dtype=np.int64)
     beyond = np.maximum((q * group + 15) // 16 - FP4_BLOCK_TILES, 0)
     if not beyond.any():
         return FP4_BLOCK_TILES + 1
     reach = np.minimum(c, window + q) if window else c
-    return FP4_BLOCK_TILES if int((beyond * reach).sum()) >= FP4_BLOCK_WORK else 1 << 30
+    if int((beyond * reach).sum()) < FP4_BLOCK_WORK:
+        return 1 << 30
+    if most_unpacked is None:
+        return FP4_BLOCK_TILES
+    first, until = _pages_read(q, c, window, page)
+    tokens = np.where((q * group + 15) // 16 >= FP4_BLOCK_TILES, (until - first) * page, 0)
+    if int(tokens.sum()) <= most_unpacked:
+        return FP4_BLOCK_TILES
+    needed, left = np.full(q.size, 1 << 30, dtype=np.int64), most_unpacked
+    for i in np.argsort(-beyond * reach, kind="stable").tolist():
+        if tokens[i] <= left:
+            needed[i] = FP4_BLOCK_TILES
+            left -= int(tokens[i])
+    return needed
+
+
+def _pages_read(q_len, ctx_len, window: int, page: int):
+    """Per item the block-table columns [first, until) that its rows read."""
+    low = np.maximum(0, ctx_len - q_len - window + 1) if window else np.zeros_like(ctx_len)
+    return low // page, -(-ctx_len // page)
 
 
 FP4_HEAD_DIMS = (64, 128, 256)      # head sizes that the 4-bit attention kernel is built for
 
 
-def fp4_unpack_list(q_len, ctx_len, group: int, head_dim: int, page: int, window: int, only_blocks: bool):
+def fp4_unpack_list(q_len, ctx_len, group: int, head_dim: int, page: int, window: int, only_blocks: bool,
+                    most_unpacked: int | None = None):
     """Which pages of a 4-bit cache a step reads through unpacked copies (those of the block kernel's items, or of all):
     int32 ``[n, 2]`` (item, column of the block table), and int32 ``[items, columns]`` where each lies among them."""
     q_len, ctx_len = np.asarray(q_len, dtype=np.int64), np.asarray(ctx_len, dtype=np.int64)
-    chosen = (items_in_blocks(q_len, group, head_dim, fp4_block_tiles(q_len, ctx_len, group, window)) if only_blocks
-              else np.ones(q_len.size, dtype=bool))
-    low = np.maximum(0, ctx_len - q_len - window + 1) if window else np.zeros_like(ctx_len)
-    first, until = low // page, -(-ctx_len // page)
+    chosen = (items_in_blocks(q_len, group, head_dim, fp4_block_tiles(q_len, ctx_len, group, window, page, most_unpacked))
+              if only_blocks else np.ones(q_len.size, dtype=bool))
+    first, until = _pages_read(q_len, ctx_len, window, page)
     column = np.arange(int(until.max()))[None, :]
     read = (column >= first[:, None]) & (column < until[:, None]) & chosen[:, None]
     pairs = np.ascontiguousarray(np.argwhere(read), dtype=np.int32)
@@ -176,8 +199,9 @@ def fp4_unpack_list(q_len, ctx_len, group: int, head_dim: int, page: int, window
     return pairs, table
 
 
-def items_in_blocks(q_len, group: int, head_dim: int, block_tiles: int = TILES_PER_BLOCK // 2) -> np.ndarray:
-    """Which items go to the block kernel: those with at least half a block of tiles, or ``block_tiles``."""
+def items_in_blocks(q_len, group: int, head_dim: int, block_tiles=TILES_PER_BLOCK // 2) -> np.ndarray:
+    """Which items go to the block kernel: those with at least half a block of tiles, or ``block_tiles`` (a number, or one
+    for each item)."""
     tiles = (np.asarray(q_len, dtype=np.int64) * group + 15) // 16
     if not head_dim or head_dim % 32 or head_dim > TILED_MAX_HEAD_DIM:
         return np.zeros(tiles.size, dtype=bool)
@@ -186,7 +210,7 @@ def items_in_blocks(q_len, group: int, head_dim: int, block_tiles: int = TILES_P
 
 def build_attention_work_numpy(q_len, ctx_len, group: int, kv_heads: int, window: int = 0,
                                target_waves: int = TARGET_WAVES, head_dim: int = 0,
-                               min_split_keys: int = MIN_SPLIT_KEYS, block_tiles: int = TILES_PER_BLOCK // 2) -> AttentionWork:
+                               min_split_keys: int = MIN_SPLIT_KEYS, block_tiles=TILES_PER_BLOCK // 2) -> AttentionWork:
     """``head_dim``: 0 keeps every item on the one-wavefront kernel (callers that do not know it).
 
     Items with at least half a block of tiles (prompt portions) go to the block kernel, the others

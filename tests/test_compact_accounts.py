@@ -9,6 +9,7 @@ from sparseengine_amd import LLM, SamplingParams
 from sparseengine_amd.cache.manager import bytes_per_token
 from sparseengine_amd.config.method_registry import PassThroughMethod
 from sparseengine_amd.engine.runner import ModelRunner
+from sparseengine_amd.kernels import attention_work as aw
 from sparseengine_amd.parts.base import PagedKVRequest
 from tests.helpers import make_folder, random_tokens
 from tests.twin_kernels import TwinKernels
@@ -118,3 +119,54 @@ def test_memory_kept_for_unpacked_pages(monkeypatch, dtype, head_dim, direct, la
     at_once = 2 * 4096 if direct else tokens
     assert tokens * held + at_once * unpacked <= usable          # and no more is left unused than a token of each
     assert (tokens + 1) * held + (at_once + (not direct)) * unpacked > usable
+
+
+def test_portions_of_many_prompts_unpack_no_more_than_they_may():
+    """Of the items that would go in blocks the heaviest do, as far as the limit reaches; the others keep the 4-bit kernel,
+    the list of pages is that of the items in blocks, and both builders agree."""
+    rng = np.random.default_rng(3)
+    limited = 0
+    for _ in range(200):
+        n = int(rng.integers(1, 12))
+        ctx = rng.integers(1, 20000, n)
+        q = np.minimum(rng.integers(1, 400, n), ctx)
+        group, window, page = int(rng.choice([1, 6, 16])), int(rng.choice([0, 0, 3000])), int(rng.choice([32, 64, 96]))
+        most = int(rng.integers(1, 80000))
+        work = aw.build_fp4_attention_work(q, ctx, group, 8, window, 128, page, most)
+        free = aw.build_fp4_attention_work(q, ctx, group, 8, window, 128)
+        pairs, table = aw.fp4_unpack_list(q, ctx, group, 128, page, window, True, most)
+        items, all_items = set(work.block_units[:, 0].tolist()), set(free.block_units[:, 0].tolist())
+        assert len(pairs) * page <= most and set(pairs[:, 0].tolist()) == items and items <= all_items
+        assert items | set(work.units[:, 0].tolist()) == set(range(n))
+        limited += items != all_items
+        held = -(-ctx // page) - (np.maximum(0, ctx - q - window + 1) // page if window else 0)
+        if sum(int(held[i]) for i in all_items) * page <= most:
+            assert items == all_items
+        for i in all_items - items:       # what was left out would not have fitted beside those that are in
+            assert (len(pairs) + int(held[i])) * page > most
+        tiles = aw.fp4_block_tiles(q, ctx, group, window, page, most)
+        a = aw.build_attention_work(q, ctx, group, 8, window, 900, 128, 64, tiles)
+        b = aw.build_attention_work_numpy(q, ctx, group, 8, window, 900, 128, 64, tiles)
+        assert all((getattr(a, f) == getattr(b, f)).all() for f in ("units", "tasks", "block_units")) and a.num_slots == b.num_slots
+    assert limited > 20
+
+
+def test_the_engine_limits_what_a_step_unpacks():
+    """Four portions on long prefixes in one step: the batch's list of pages holds two longest prompts' tokens at most."""
+    from sparseengine_amd.cache.manager import CacheManager
+    from sparseengine_amd.engine.batch import BatchBuilder, StepItem
+    cache = CacheManager({0: PagedKVRequest(1, 64, None, None)}, max_rows=4, max_model_len=40000, page_size=64, num_tokens=4 * 40000,
+                         dtype=torch.bfloat16, device="cpu", kv_dtype=torch.uint8)
+    rows = [cache.admit(i) for i in range(4)]
+    cache.append([(row, 38000) for row in rows])
+    builder = BatchBuilder(None, cache, torch.bfloat16, "cpu", 512, attention_shapes={0: {(16, 0)}}, most_unpacked=2 * 40000)
+    fb = builder.build([StepItem(row, [1] * 64, [63]) for row in rows])
+    work, (pairs, table) = fb.groups[0].work[(16, 0, "fp4")], fb.groups[0].work[("unpack", 16, 64, 64, 0, True)]
+    assert pairs.shape[0] * 64 <= 80000 and len(set(pairs[:, 0].tolist())) == 2
+    assert set(work.block_units[:, 0].tolist()) == set(pairs[:, 0].tolist())
+    assert set(work.block_units[:, 0].tolist()) | set(work.units[:, 0].tolist()) == {0, 1, 2, 3}
+
+
+def test_the_runner_limits_its_batches(tmp_path):
+    llm = evicting(tmp_path, max_model_len=160)
+    assert llm.runner.builder.most_unpacked == 2 * 160
