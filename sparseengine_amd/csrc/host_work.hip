@@ -20,7 +20,8 @@ constexpr int BLOCK_UNIT_FIELDS = 12;
 
 struct Rules {  // order of the `rules` argument
   int64_t target_waves, min_split_keys, max_splits, tiles_per_block, tiled_max_head_dim, target_blocks,
-      min_block_keys, prefix_per_portion;
+      min_block_keys, prefix_per_portion,
+      most_keys;      // of a wavefront's range where the wavefronts fill the chip without ranges
 };
 
 // per item: in_blocks, rows (tiles or blocks), splits, chunk, first_key, base
@@ -29,10 +30,10 @@ constexpr int PLAN_FIELDS = 6;
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int64_t keys_per_unit(const std::vector<int64_t>& units_per_item, const std::vector<int64_t>& reach,
-                      int kv_heads, int64_t wanted, int64_t least) {
+                      int kv_heads, int64_t wanted, int64_t least, int64_t most) {
   int64_t in_flight = 0, ranges_at_least = 0, keys = 0;
   for (size_t i = 0; i < reach.size(); ++i) in_flight += units_per_item[i];
-  if (in_flight * kv_heads >= wanted) return int64_t(1) << 30;
+  if (in_flight * kv_heads >= wanted) return most;
   for (size_t i = 0; i < reach.size(); ++i) ranges_at_least += units_per_item[i] * (reach[i] / least);
   if (ranges_at_least * kv_heads < wanted / 2) least = std::max<int64_t>(32, least / 2);
   for (size_t i = 0; i < reach.size(); ++i) keys += units_per_item[i] * reach[i];
@@ -50,7 +51,8 @@ int se_attention_work_plan(const int64_t* q_len, const int64_t* ctx_len, int ite
                            int kv_heads, int window, int head_dim, const int64_t* block_tiles, const int64_t* rules_in,
                            int64_t* plan, int64_t* counts) {
   if (items < 0 || group <= 0 || kv_heads <= 0) return -1;
-  Rules r{rules_in[0], rules_in[1], rules_in[2], rules_in[3], rules_in[4], rules_in[5], rules_in[6], rules_in[7]};
+  Rules r{rules_in[0], rules_in[1], rules_in[2], rules_in[3], rules_in[4], rules_in[5], rules_in[6], rules_in[7],
+          rules_in[8]};
   const bool blocks_allowed = head_dim > 0 && head_dim % 32 == 0 && head_dim <= r.tiled_max_head_dim;
   std::vector<int64_t> tiles(items), reach(items), nblocks(items), alone(items), cut_blocks(items);
   int64_t whole = 0;      // blocks of items that are never cut into key ranges
@@ -69,9 +71,9 @@ int se_attention_work_plan(const int64_t* q_len, const int64_t* ctx_len, int ite
   }
   whole *= kv_heads;
   const int64_t block_keys = r.target_blocks > whole
-      ? keys_per_unit(cut_blocks, reach, kv_heads, r.target_blocks - whole, r.min_block_keys)
+      ? keys_per_unit(cut_blocks, reach, kv_heads, r.target_blocks - whole, r.min_block_keys, int64_t(1) << 30)
       : int64_t(1) << 30;
-  const int64_t wave_keys = keys_per_unit(alone, reach, kv_heads, r.target_waves, r.min_split_keys);
+  const int64_t wave_keys = keys_per_unit(alone, reach, kv_heads, r.target_waves, r.min_split_keys, r.most_keys);
   int64_t units = 0, tasks = 0, blocks = 0, slots = 0;
   for (int i = 0; i < items; ++i) {
     const bool in_blocks = plan[i * PLAN_FIELDS + 0] != 0;

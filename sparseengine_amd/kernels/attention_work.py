@@ -38,6 +38,7 @@ TILED_MAX_HEAD_DIM = 128
 TARGET_BLOCKS = 1536   # blocks wanted in flight (three rounds of two per CU); fewer: their keys are split
 MIN_BLOCK_KEYS = 2048
 PREFIX_PER_PORTION = 3
+WHOLE = 1 << 30        # more keys than any context: not cut into ranges
 
 
 @dataclass
@@ -75,6 +76,11 @@ FP4_WAVES = 1024            # ranges wanted at head sizes from 128 on, while the
 FP4_MANY_WAVES = 2048       # else
 FP4_MIN_SPLIT_KEYS = 128
 FP4_WHOLE_KEYS = 160        # a step none of whose contexts is longer is not split at all
+# Where the tiles alone fill the chip, a range holds at most so many times the mean keys of a tile: 200 requests of 500 keys
+# and one of 131071 take 92 us instead of 2302 us, in which one wavefront per kv head goes through all of the long one; 300 of
+# 2000 and the same one 201 instead of 2369 us; 200 of 3000 and four of 12000 177 instead of 274 us.  Lengths within twice
+# their mean, the ordinary step, are not cut (160 of 4000 to 8200: 273 us).
+FP4_MOST_MEANS = 2
 # Items in blocks read unpacked pages, which takes a launch and writes and reads four times the bytes, but then every
 # product costs less than half: 5.6 against about 2.5 us a row tile and 32768 keys (48:8 heads of 128, one request).  16,
 # 64, 128 and 192 rows at 4096 keys take 48, 55, 59 and 63 us in blocks, 18, 32, 52 and 69 directly; 16, 32 and 128 at
@@ -108,14 +114,15 @@ _BAD_LENGTHS = "attention work: every item needs at least one new token and no m
 
 def build_attention_work(q_len, ctx_len, group: int, kv_heads: int, window: int = 0,
                          target_waves: int = TARGET_WAVES, head_dim: int = 0,
-                         min_split_keys: int = MIN_SPLIT_KEYS, block_tiles=TILES_PER_BLOCK // 2) -> AttentionWork:
+                         min_split_keys: int = MIN_SPLIT_KEYS, block_tiles=TILES_PER_BLOCK // 2,
+                         most_keys: int = WHOLE) -> AttentionWork:
     """The work lists of one step, from the compiled builder; ``build_attention_work_numpy`` states
     the rules and gives the same lists (the tests compare the two), about twenty times slower."""
     lib = _native_library()
     q = np.ascontiguousarray(q_len, dtype=np.int64)
     c = np.ascontiguousarray(ctx_len, dtype=np.int64)
     rules = np.asarray([target_waves, min_split_keys, MAX_SPLITS, TILES_PER_BLOCK, TILED_MAX_HEAD_DIM,
-                        TARGET_BLOCKS, MIN_BLOCK_KEYS, PREFIX_PER_PORTION], dtype=np.int64)
+                        TARGET_BLOCKS, MIN_BLOCK_KEYS, PREFIX_PER_PORTION, most_keys], dtype=np.int64)
     needed = np.full(q.size, block_tiles, dtype=np.int64)      # a number for all items, or one for each
     plan = np.empty((q.size, 6), dtype=np.int64)
     counts = np.empty(4, dtype=np.int64)
@@ -141,12 +148,18 @@ def build_fp4_attention_work(q_len, ctx_len, group: int, kv_heads: int, window: 
     item's last range is a partial one, so one is taken off the number wanted for each tile)."""
     q = np.asarray(q_len, dtype=np.int64)
     block_tiles = fp4_block_tiles(q, ctx_len, group, window, page, most_unpacked)
-    tiles = int(((q * group + 15) // 16)[~items_in_blocks(q, group, head_dim, block_tiles)].sum()) * kv_heads
+    alone = np.where(items_in_blocks(q, group, head_dim, block_tiles), 0, (q * group + 15) // 16)
+    tiles = int(alone.sum()) * kv_heads
     wanted = FP4_WAVES if head_dim >= 128 and 4 * tiles <= FP4_WAVES else FP4_MANY_WAVES
     if q.size and int(np.max(ctx_len)) <= FP4_WHOLE_KEYS:
         wanted = 0
+    most = WHOLE
+    if tiles >= wanted - tiles and tiles:      # no ranges are wanted: an item far above the others gets some all the same
+        c = np.asarray(ctx_len, dtype=np.int64)
+        mean = -(-int((alone * (np.minimum(c, window + q) if window else c)).sum()) * kv_heads // tiles)
+        most = max(FP4_WHOLE_KEYS, -(-FP4_MOST_MEANS * mean // 32) * 32)
     return build_attention_work(q_len, ctx_len, group, kv_heads, window, max(1, wanted - tiles), head_dim, FP4_MIN_SPLIT_KEYS,
-                                block_tiles)
+                                block_tiles, most)
 
 
 def fp4_block_tiles(q_len, ctx_len, group: int, window: int, page: int = 1, most_unpacked: int | None = None):
@@ -210,13 +223,15 @@ def items_in_blocks(q_len, group: int, head_dim: int, block_tiles=TILES_PER_BLOC
 
 def build_attention_work_numpy(q_len, ctx_len, group: int, kv_heads: int, window: int = 0,
                                target_waves: int = TARGET_WAVES, head_dim: int = 0,
-                               min_split_keys: int = MIN_SPLIT_KEYS, block_tiles=TILES_PER_BLOCK // 2) -> AttentionWork:
+                               min_split_keys: int = MIN_SPLIT_KEYS, block_tiles=TILES_PER_BLOCK // 2,
+                               most_keys: int = WHOLE) -> AttentionWork:
     """``head_dim``: 0 keeps every item on the one-wavefront kernel (callers that do not know it).
 
     Items with at least half a block of tiles (prompt portions) go to the block kernel, the others
     keep one wavefront per tile.  In both classes the keys are cut into ranges when the class alone
     would not fill the chip; the number of ranges of an item follows its context, so that a long
-    context beside short ones does not become the one long-running unit."""
+    context beside short ones does not become the one long-running unit.  Where the single wavefronts fill the chip
+    without ranges, ``most_keys`` is the most that one of them goes through."""
     q_len = np.asarray(q_len, dtype=np.int64)
     ctx_len = np.asarray(ctx_len, dtype=np.int64)
     if ((q_len < 1) | (q_len > ctx_len)).any():
@@ -226,11 +241,11 @@ def build_attention_work_numpy(q_len, ctx_len, group: int, kv_heads: int, window
     reach = np.minimum(ctx_len, window + q_len) if window else ctx_len      # keys an item's tiles can read
     in_blocks = items_in_blocks(q_len, group, head_dim, block_tiles)
 
-    def keys_per_unit(units_per_item, wanted: int, least: int) -> int:
+    def keys_per_unit(units_per_item, wanted: int, least: int, most: int = WHOLE) -> int:
         """Keys of a range so that all ranges together number about ``wanted``."""
         in_flight = int(units_per_item.sum()) * kv_heads
         if in_flight >= wanted:
-            return 1 << 30
+            return most
         if int((units_per_item * (reach // least)).sum()) * kv_heads < wanted // 2:
             least = max(32, least // 2)
         share = -(-int((units_per_item * reach).sum()) * kv_heads // wanted)
@@ -243,7 +258,7 @@ def build_attention_work_numpy(q_len, ctx_len, group: int, kv_heads: int, window
     cut = in_blocks & (reach - q_len >= PREFIX_PER_PORTION * q_len)
     whole = int(np.where(cut, 0, nblocks).sum()) * kv_heads
     block_keys = keys_per_unit(np.where(cut, nblocks, 0), TARGET_BLOCKS - whole, MIN_BLOCK_KEYS) if TARGET_BLOCKS > whole else 1 << 30
-    keys = np.where(in_blocks, np.where(cut, block_keys, 1 << 30), keys_per_unit(alone, target_waves, min_split_keys))
+    keys = np.where(in_blocks, np.where(cut, block_keys, 1 << 30), keys_per_unit(alone, target_waves, min_split_keys, most_keys))
     # equal ranges (multiples of 32 keys) over [first_key, ctx) of every item
     first_key = np.maximum(0, ctx_len - reach) // 32 * 32
     span = ctx_len - first_key

@@ -170,3 +170,27 @@ def test_the_engine_limits_what_a_step_unpacks():
 def test_the_runner_limits_its_batches(tmp_path):
     llm = evicting(tmp_path, max_model_len=160)
     assert llm.runner.builder.most_unpacked == 2 * 160
+
+
+def test_a_long_context_beside_many_short_ones_is_cut():
+    """Where the tiles alone fill the chip, an item of more than twice the mean keys is cut all the same: no wavefront goes
+    through a whole long context by itself.  Items near the mean, and short ones, stay whole."""
+    longest = lambda work: int((work.units[:, 3] - work.units[:, 2]).max())
+    for short, many in ((500, 100), (500, 200), (2000, 300), (70, 1000)):
+        ctx = [short] * many + [131071]
+        work = aw.build_fp4_attention_work([1] * len(ctx), ctx, 6, 8, 0, 128)
+        mean = -(-sum(ctx) // len(ctx))
+        assert longest(work) <= max(aw.FP4_WHOLE_KEYS, 2 * mean + 32, 131071 // aw.MAX_SPLITS + 32)
+        assert set(work.tasks[:, 0].tolist()) == {many} or many == 100
+        for item, n in ((0, short), (many, 131071)):      # every key once
+            mine = work.units[work.units[:, 0] == item]
+            assert mine[0, 2] == 0 and mine[-1, 3] == n and (mine[1:, 2] == mine[:-1, 3]).all()
+        numpy = aw.build_attention_work_numpy([1] * len(ctx), ctx, 6, 8, 0, 1, 128, 128, 9, 2 * mean // 32 * 32)
+        native = aw.build_attention_work([1] * len(ctx), ctx, 6, 8, 0, 1, 128, 128, 9, 2 * mean // 32 * 32)
+        assert (numpy.units == native.units).all() and (numpy.tasks == native.tasks).all()
+    rng = np.random.default_rng(0)
+    near = rng.integers(4000, 8200, 160)
+    assert len(aw.build_fp4_attention_work([1] * 160, near, 6, 8, 0, 128).tasks) == 0
+    assert len(aw.build_fp4_attention_work([1] * 300, [20] * 299 + [160], 6, 8, 0, 128).tasks) == 0
+    # a window leaves nothing long
+    assert len(aw.build_fp4_attention_work([1] * 201, [500] * 200 + [131071], 6, 8, 600, 128).tasks) == 0
