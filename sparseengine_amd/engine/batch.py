@@ -16,7 +16,7 @@ import torch
 
 from ..cache.manager import CacheManager
 from ..kernels.attention_work import (FP4_HEAD_DIMS, DeviceAttentionWork, build_attention_work, build_fp4_attention_work,
-                                      fp4_unpack_list)
+                                      fp4_unpack_list, step_lengths)
 from ..parts.base import StepScratch
 
 
@@ -45,7 +45,8 @@ class GroupMeta:
     max_ctx_len: int = 0
     max_q_len: int = 0
     # (query heads per kv head, window) -> (units, num_units, tasks, num_tasks, partial slots) of
-    # the matrix-core attention kernel, prepared with the rest of the step's integers
+    # the matrix-core attention kernel, prepared with the rest of the step's integers; for a cache in 4 bits also the
+    # lengths that they are for (attention_work.py: StepLengths) and the lists of pages to unpack
     work: dict = field(default_factory=dict)
 
 
@@ -268,6 +269,10 @@ class BatchBuilder:
                 page_size=group.page_size, item_q_start=q_start, item_q_len=q_len,
                 item_ctx_len=ctx_len, item_meta=item_meta, max_ctx_len=int(ctx_len.max()),
                 max_q_len=int(q_len.max()))
+        if works and cache.kv_dtype == torch.uint8:
+            lengths = step_lengths(q_len, ctx_len)
+            for group in cache.groups:
+                fb.groups[group.index].work["lengths"] = lengths
         for group_index, key, work, at in works:
             fb.groups[group_index].work[key] = DeviceAttentionWork(
                 view(at, work.units.shape), work.units.shape[0], view(at + 1, work.tasks.shape),

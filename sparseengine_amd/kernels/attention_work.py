@@ -65,6 +65,27 @@ class DeviceAttentionWork:
     tiles_per_block: int
 
 
+@dataclass
+class StepLengths:
+    """The lengths that a step's kept work lists are for (under ``"lengths"`` among them)."""
+    q_len: object            # ``lengths_key`` of the items' new tokens
+    ctx_len: object          # and of their contexts
+    numbers: bytes           # both, whatever kind of sequence they came in
+    tokens: int              # of the step
+    items: int
+    longest: int             # context
+
+
+def lengths_key(lengths):
+    """What two equal sequences of lengths of one kind have in common."""
+    return lengths.tobytes() if type(lengths) is np.ndarray else tuple(lengths)
+
+
+def step_lengths(q_len, ctx_len) -> StepLengths:
+    both = np.asarray([q_len, ctx_len], dtype=np.int64)
+    return StepLengths(lengths_key(q_len), lengths_key(ctx_len), both.tobytes(), int(both[0].sum()), both.shape[1], int(both[1].max()))
+
+
 # A cache in 4 bits (the same heads; the kernel alone would be bound by reading at one wavefront per SIMD, and a few
 # too many, which run beside the others on some SIMDs, cost as much as twice as many everywhere).  4 requests of up to
 # 131071 keys take 70 us in at most 1024 ranges (6.1 TB/s in the kernel), 78 us in 2048, 85 us in 768; 16 x 16384 keys 44

@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from . import library
-from .attention_work import FP4_HEAD_DIMS, fp4_unpack_list
+from .attention_work import FP4_HEAD_DIMS, fp4_unpack_list, lengths_key, step_lengths
 
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
 
@@ -512,6 +512,11 @@ class HipKernels:
         page = self._fp4_cache(cache, head_dim)
         kv_heads = cache.shape[2]
         self._check_items(meta, tokens, page, "attention over a 4-bit cache")
+        if getattr(meta, "work", None) is not None:      # lists kept for other lengths would send the kernels to other pages
+            now = step_lengths(meta.item_q_len, meta.item_ctx_len)
+            _require(meta.work.get("lengths", now).numbers == now.numbers,
+                     "attention over a 4-bit cache: the work lists kept in meta.work are those of other lengths")
+            meta.work["lengths"] = now
         _require(scale > 0, "attention over a 4-bit cache: scale must be positive")
         direct = q.dtype == torch.bfloat16 and head_dim in FP4_HEAD_DIMS
         group = heads // kv_heads
@@ -675,7 +680,8 @@ class HipKernels:
         page_size, head_dim * 17 / 32]``, cache/layout.py): ``meta`` then needs its items, ``scale`` is positive, ``window`` not negative, and
         the call allocates what its longer way needs: partial results, and for the portions of prompts that it reads
         through unpacked pages a copy of those in ``q``'s type.  A key or value that is not a number reaches the rows that
-        see it and no others; over unpacked pages in bfloat16 all dims of theirs, else the value's groups of 32."""
+        see it and no others; over unpacked pages in bfloat16 all dims of theirs, else the value's groups of 32.
+        The first call on a meta leaves its lists in ``meta.work``, if it has one; they are for the lengths of that call."""
         tokens, heads, head_dim = q.shape
         kv_heads, page_size = cache.shape[2], cache.shape[3]
         _require(q.stride(2) == 1 and q.stride(1) == head_dim, "q heads must be dense")
@@ -684,14 +690,17 @@ class HipKernels:
             # a step of few rows per item with its work list prepared, in one expression; every other call, and one that
             # fails a check, takes the long way, which names what is wrong
             work, table = meta.work.get((heads // kv_heads if kv_heads else 0, window, "fp4")), meta.block_table
-            if (work is not None and not work.num_block_units and 0 <= window <= 0x7fffffff and heads % kv_heads == 0 and scale > 0
+            step = meta.work.get("lengths")
+            if (work is not None and step is not None and not work.num_block_units and 0 <= window <= 0x7fffffff and heads % kv_heads == 0
+                    and scale > 0 and step.q_len == lengths_key(meta.item_q_len) and step.ctx_len == lengths_key(meta.item_ctx_len)
                     and q.dtype == torch.bfloat16 and head_dim in FP4_HEAD_DIMS and q.stride(0) % 8 == 0
                     and cache.dim() == 5 and cache.shape[1] == 2 and cache.shape[4] * 32 == head_dim * 17 and page_size % 32 == 0
                     and cache.is_contiguous()
                     and (lse is None or lse.dtype == torch.float32 and lse.is_contiguous() and lse.shape == (tokens, heads))
                     and out.shape == (tokens, heads * head_dim) and out.stride(1) == 1 and out.dtype == torch.bfloat16
                     and out.stride(0) % 8 == 0 and table.dtype == torch.int32 and table.dim() == 2 and table.stride(1) == 1
-                    and meta.token_row.numel() == tokens and not (q.data_ptr() | cache.data_ptr() | out.data_ptr()) & 15):
+                    and step.items <= table.shape[0] and step.longest <= table.shape[1] * page_size
+                    and step.tokens == tokens == meta.token_row.numel() and not (q.data_ptr() | cache.data_ptr() | out.data_ptr()) & 15):
                 _same_device(q, cache, out, lse, table)
                 return self._run_attention_work(q, None, None, work, out, scale, window, lse, fp4=(cache, table))
         _require(fp4 or (cache.dim() == 5 and cache.shape[1] == 2 and cache.shape[4] == head_dim

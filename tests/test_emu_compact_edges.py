@@ -33,3 +33,9 @@ def test_weights_refuse_a_scale_that_is_not_positive():
         for kind in ("fp4", "own"):
             for dtype in (G.BF16, G.F32):
                 G.test_weights_refuse_a_scale_that_is_not_positive(hip, kind, dtype)
+
+
+@pytest.mark.parametrize("dtype,d", [(G.BF16, 64), (G.BF16, 96), (G.F32, 64)])
+def test_kept_work_lists_belong_to_their_lengths(guard, dtype, d):
+    with Emulated(guard=guard) as hip:
+        G.test_kept_work_lists_belong_to_their_lengths(hip, dtype, d)

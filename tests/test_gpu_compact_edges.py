@@ -1,5 +1,8 @@
 """Calls of the cache in 4 bits, of gathered weights and of eviction at the ends of what their arguments may be, against the
 plain forms of tests/compact_oracle.py (tolerances: tests/test_gpu_compact_cache.py)."""
+from types import SimpleNamespace
+
+import numpy as np
 import pytest
 import torch
 
@@ -66,3 +69,28 @@ def test_weights_refuse_a_scale_that_is_not_positive(hip, kind, dtype):
         with pytest.raises(ValueError, match="scale"):
             hip.attention_weights(q.to(C.DEV), cache.to(C.DEV), meta, torch.zeros(5, 6).to(C.DEV), weights, scale)
     assert (weights == 9).all()
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 64), (BF16, 96), (F32, 64)])
+def test_kept_work_lists_belong_to_their_lengths(hip, dtype, d):
+    """The lists that a first call leaves in ``meta.work`` are those of its lengths: calls on other ones, on a table that is
+    too narrow or has too few rows, are refused as they are without a list; the same lengths in another array go on."""
+    ctx, new = [70, 200], [1, 3]
+    meta, cache, q, of = C.attention_case("fp4", dtype, 6, 1, d, 32, ctx, new, 0)
+    cache, q = cache.to(C.DEV), q.to(C.DEV)
+    out, lse = torch.empty(4, 6 * d, dtype=dtype).to(C.DEV), torch.empty(4, 6).to(C.DEV)
+    attend = lambda m, rows=4: hip.paged_attention(q[:rows], cache, m, out[:rows], d ** -0.5, lse=lse[:rows])
+    for turn in range(2):
+        attend(meta)
+        C.check_attention(out, lse, q.cpu(), of, ctx, new, d ** -0.5, 0, dtype)
+        with_ = lambda **k: SimpleNamespace(**{**vars(meta), **k})
+        for bad in (dict(item_ctx_len=np.asarray([70, 199])), dict(item_ctx_len=np.asarray([200, 70])), dict(item_q_len=np.asarray([2, 2])),
+                    dict(block_table=meta.block_table[:, :6].contiguous()), dict(block_table=meta.block_table[:1].contiguous()),
+                    dict(item_q_len=np.asarray([1]), item_ctx_len=np.asarray([70]))):
+            with pytest.raises(ValueError):
+                attend(with_(**bad))
+        with pytest.raises(ValueError):
+            attend(with_(token_row=meta.token_row[:3], positions=meta.positions[:3]), 3)
+        for same in (lambda a: a.copy(), list, lambda a: a.astype(np.int32)):
+            attend(with_(item_q_len=same(meta.item_q_len), item_ctx_len=same(meta.item_ctx_len)))
+        C.check_attention(out, lse, q.cpu(), of, ctx, new, d ** -0.5, 0, dtype)
