@@ -96,7 +96,8 @@ class ModelRunner:
         self.model = arch.make_model(self.spec, chunk_tokens=mlp_chunk_size)
         if getattr(kernels, "libraries", None):
             from ..kernels import library
-            library.ensure_built(sorted(self.model.all_kernel_libraries() | set(self.method.kernel_libraries)))
+            compact = {"cache_fp4", "attention_fp4"} if self.kv_dtype == torch.uint8 else set()
+            library.ensure_built(sorted(self.model.all_kernel_libraries() | set(self.method.kernel_libraries) | compact))
         self.max_model_len = int(max_model_len or self.spec.max_position)
         if self.max_model_len > self.spec.max_position:
             raise ValueError(f"max_model_len {self.max_model_len} exceeds the model's "

@@ -117,7 +117,7 @@ _SIGNATURES = {
     "cache_fp4": {
         # qkv, row_stride, slots, tokens, heads, kv_heads, head_dim, cache, page_size, dtype, stream
         "se_fp4_store": [c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p],
-        # cache, pages, bt_stride, list, count, out, kv_heads, page_size, head_dim, dtype, stream
+        # cache, pages, bt_stride, list, count, out, kv_heads, page_size, head_dim, dtype, for_products, stream
         "se_fp4_unpack": [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
     },
     "attention_weights": {

@@ -11,6 +11,7 @@ from sparseengine_amd.config.method_registry import PassThroughMethod
 from sparseengine_amd.engine.runner import ModelRunner
 from sparseengine_amd.kernels import attention_work as aw
 from sparseengine_amd.parts.base import PagedKVRequest
+from tests import backends
 from tests.helpers import make_folder, random_tokens
 from tests.twin_kernels import TwinKernels
 
@@ -194,3 +195,16 @@ def test_a_long_context_beside_many_short_ones_is_cut():
     assert len(aw.build_fp4_attention_work([1] * 300, [20] * 299 + [160], 6, 8, 0, 128).tasks) == 0
     # a window leaves nothing long
     assert len(aw.build_fp4_attention_work([1] * 201, [500] * 200 + [131071], 6, 8, 600, 128).tasks) == 0
+
+
+@pytest.mark.skipif(not backends.EmulatedBackend().available(), reason="no host compiler for the emulated kernels")
+@pytest.mark.parametrize("kwargs,more", [({}, set()), (dict(kv_cache_dtype="fp4", kv_page_size=32), {"cache_fp4", "attention_fp4"}),
+                                         (dict(sparse_method="accumulated_weight", eviction_budget=8), {"attention_weights", "evict"})])
+def test_only_the_libraries_that_are_called_are_built(tmp_path, monkeypatch, kwargs, more):
+    from sparseengine_amd.kernels import library
+    asked = []
+    monkeypatch.setattr(library, "ensure_built", lambda names=None, *a, **k: asked.append(set(names)))
+    with backends.use(backends.EmulatedBackend()) as backend:
+        LLM(make_folder(tmp_path, "C_loud"), num_kvcache_slots=128, **kwargs, **backend.llm_kwargs())
+    compact = {"cache_fp4", "attention_fp4", "attention_weights", "evict"}
+    assert asked[0] & compact == more and {"rope_kv", "attention_mfma", "norm"} <= asked[0]
