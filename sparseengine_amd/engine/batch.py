@@ -139,6 +139,9 @@ class BatchBuilder:
         self.kernels, self.cache, self.dtype, self.device = kernels, cache, dtype, torch.device(device)
         self.vocab_size = vocab_size
         self.attention_shapes = attention_shapes or {}
+        # a method's own cache manager need not know of evicted tokens or of a layer type apart from the engine's
+        self.row_dropped = getattr(cache, "row_dropped", None)
+        self.kv_dtype = getattr(cache, "kv_dtype", dtype)
         self.most_unpacked = most_unpacked
         self.scratch = StepScratch()
         self._host = None
@@ -152,6 +155,11 @@ class BatchBuilder:
             self._host = torch.empty(size, dtype=torch.int32, pin_memory=pin)
             self._dev = torch.empty(size, dtype=torch.int32, device=self.device)
         return self._host, self._dev
+
+    def _dropped(self, rows):
+        """Evicted tokens of the rows, None if there are none."""
+        dropped = None if self.row_dropped is None else self.row_dropped[rows]
+        return dropped if dropped is not None and dropped.any() else None
 
     def build(self, items: list[StepItem]) -> ForwardBatch:
         if not items:
@@ -172,12 +180,12 @@ class BatchBuilder:
                 if it.want and any(w != 0 for w in it.want):
                     raise ValueError("a wanted place lies outside the item's tokens")
             places = cache.row_len[rows].astype(np.int32)
-            dropped = cache.row_dropped[rows]
+            dropped = self._dropped(rows)
             allocation = cache.append([(it.row, 1) for it in items])   # all or nothing
             q_start = token_item = np.arange(B, dtype=np.int32)
             q_len = np.ones(B, dtype=np.int32)
             ctx_len = places + 1
-            positions = places + dropped.astype(np.int32) if dropped.any() else places
+            positions = places if dropped is None else places + dropped.astype(np.int32)
             want = np.asarray([i for i, it in enumerate(items) for _ in it.want], dtype=np.int32)
         else:
             for it in items:
@@ -196,8 +204,8 @@ class BatchBuilder:
             ctx_len = np.asarray([s + n for s, n in zip(starts, lengths)], dtype=np.int32)
             token_ids = np.concatenate([np.asarray(it.tokens, dtype=np.int32) for it in items])
             places = np.concatenate([np.arange(s, s + n, dtype=np.int32) for s, n in zip(starts, lengths)])
-            dropped = cache.row_dropped[[it.row for it in items]]
-            positions = places + np.repeat(dropped, lengths).astype(np.int32) if dropped.any() else places
+            dropped = self._dropped([it.row for it in items])
+            positions = places if dropped is None else places + np.repeat(dropped, lengths).astype(np.int32)
             token_item = np.repeat(np.arange(B, dtype=np.int32), lengths)
             want = np.asarray([q_start[i] + w for i, it in enumerate(items) for w in it.want], dtype=np.int32)
             rows = np.asarray([it.row for it in items], dtype=np.int32)
@@ -217,7 +225,7 @@ class BatchBuilder:
             parts.append(places)
         works, lists = [], []
         if self.attention_shapes:
-            fp4 = cache.kv_dtype == torch.uint8
+            fp4 = self.kv_dtype == torch.uint8
             for group in cache.groups:
                 head_dim = group.request.head_dim
                 direct = fp4 and self.dtype == torch.bfloat16 and head_dim in FP4_HEAD_DIMS
@@ -269,7 +277,7 @@ class BatchBuilder:
                 page_size=group.page_size, item_q_start=q_start, item_q_len=q_len,
                 item_ctx_len=ctx_len, item_meta=item_meta, max_ctx_len=int(ctx_len.max()),
                 max_q_len=int(q_len.max()))
-        if works and cache.kv_dtype == torch.uint8:
+        if works and self.kv_dtype == torch.uint8:
             lengths = step_lengths(q_len, ctx_len)
             for group in cache.groups:
                 fb.groups[group.index].work["lengths"] = lengths

@@ -208,3 +208,28 @@ def test_only_the_libraries_that_are_called_are_built(tmp_path, monkeypatch, kwa
         LLM(make_folder(tmp_path, "C_loud"), num_kvcache_slots=128, **kwargs, **backend.llm_kwargs())
     compact = {"cache_fp4", "attention_fp4", "attention_weights", "evict"}
     assert asked[0] & compact == more and {"rope_kv", "attention_mfma", "norm"} <= asked[0]
+
+
+def test_a_cache_manager_that_knows_nothing_of_eviction(tmp_path):
+    """A method's own manager with the constructor and interface of the paged one, but none of what eviction and 4 bits added
+    to it, serves the dense method as before."""
+    from sparseengine_amd.cache.manager import CacheManager
+    from sparseengine_amd.config import method_registry
+
+    class Plain:
+        def __init__(self, requests, **kwargs):
+            self.paged = CacheManager(requests, **kwargs)
+
+        def __getattr__(self, name):
+            if name in ("row_dropped", "kv_dtype", "begin_eviction", "finish_eviction", "abort_eviction"):
+                raise AttributeError(name)
+            return getattr(self.__dict__["paged"], name)
+
+    method_registry.register_method("plain", PassThroughMethod, "all_chunked", cache_manager_cls=Plain)
+    try:
+        prompts = [random_tokens(n, 512, n) for n in (20, 5)]
+        make = lambda **k: evicting(tmp_path, eviction_budget=0, **k)
+        out, dense = (make(sparse_method=name).generate(prompts, greedy(4), use_tqdm=False) for name in ("plain", ""))
+        assert [o["token_ids"] for o in out] == [o["token_ids"] for o in dense]
+    finally:
+        method_registry._METHODS.pop("plain", None)
