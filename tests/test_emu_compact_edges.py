@@ -39,3 +39,9 @@ def test_weights_refuse_a_scale_that_is_not_positive():
 def test_kept_work_lists_belong_to_their_lengths(guard, dtype, d):
     with Emulated(guard=guard) as hip:
         G.test_kept_work_lists_belong_to_their_lengths(hip, dtype, d)
+
+
+@pytest.mark.parametrize("d,items", [(128, 20), (256, 6), (128, 130), (256, 130)])
+def test_joining_ranges(d, items):
+    with Emulated() as hip:
+        G.test_joining_ranges(hip, d, items)

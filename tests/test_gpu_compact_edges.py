@@ -94,3 +94,56 @@ def test_kept_work_lists_belong_to_their_lengths(hip, dtype, d):
         for same in (lambda a: a.copy(), list, lambda a: a.astype(np.int32)):
             attend(with_(item_q_len=same(meta.item_q_len), item_ctx_len=same(meta.item_ctx_len)))
         C.check_attention(out, lse, q.cpu(), of, ctx, new, d ** -0.5, 0, dtype)
+
+
+@pytest.mark.parametrize("d,items", [(128, 20), (256, 6), (128, 130), (256, 130)])
+def test_joining_ranges(hip, d, items):
+    """Ranges joined by a block per row, and from 2048 rows on by a wavefront per row."""
+    from sparseengine_amd.kernels import attention_work as aw
+    heads, kv, page = 2, 1, 32
+    ctx = [170 + 37 * i % 130 for i in range(items)]
+    meta, cache, q, of = C.attention_case("fp4", BF16, heads, kv, d, page, ctx, [1] * items, 0)
+    tasks = len(aw.build_fp4_attention_work([1] * items, ctx, heads // kv, kv, 0, d).tasks)
+    assert tasks == items and (tasks * kv * 16 >= 2048) == (items == 130)
+    out, lse = torch.empty(items, heads * d, dtype=BF16).to(C.DEV), torch.empty(items, heads).to(C.DEV)
+    hip.paged_attention(q.to(C.DEV), cache.to(C.DEV), meta, out, d ** -0.5, lse=lse)
+    C.check_attention(out, lse, q, of, ctx, [1] * items, d ** -0.5, 0, BF16)
+
+
+@pytest.mark.skipif(backends.ACTIVE.slow, reason="more keys than the emulated backend goes through")
+@pytest.mark.parametrize("d,ctx,window,previous", [(64, [300000], 0, True), (128, [150017, 150001], 0, True), (256, [290000], 0, False),
+                                                   (128, [300000, 5], 280001, True)])
+def test_weights_of_more_keys_than_one_round(hip, d, ctx, window, previous):
+    """Single tokens on so many cached keys that a wavefront of the 4-bit kernel asks for more of them while it works (more
+    than 65536 groups of 32 keys and kv heads); the plain form in float64 on the same device."""
+    heads, kv, page, scale = 16, 8, 64, d ** -0.5
+    assert sum(-(-(min(c, window) if window else c) // 32) for c in ctx) * kv > 65536
+    meta, pages = C.oracle.step(ctx, [1] * len(ctx), page, C.DEV, np.random.default_rng(1), window=window)
+    g = torch.Generator(device=C.DEV).manual_seed(2)
+    cache = torch.randint(0, 256, (pages, 2, kv, page * d * 17 // 32), dtype=torch.uint8, device=C.DEV, generator=g)
+    cache[..., page * d // 2:] = torch.randint(124, 128, (pages, 2, kv, page * d // 32), dtype=torch.uint8, device=C.DEV, generator=g)
+    cache = cache.view(pages, 2, kv, page, -1)
+    q = torch.randn(len(ctx), heads, d, device=C.DEV, generator=g).to(BF16)
+    before = torch.rand(pages, kv, page, device=C.DEV, generator=g)
+    want, bound = torch.full_like(before, 9.0, dtype=torch.float64), torch.zeros_like(before, dtype=torch.float64)
+    lse = torch.empty(len(ctx), heads, device=C.DEV)
+    for i, n in enumerate(ctx):
+        first = max(0, n - window) if window else 0
+        at = torch.arange(first, n, device=C.DEV)
+        where = meta.block_table[i].long()[at // page]
+        for h in range(kv):
+            k = C.layout.fp4_read(cache[:, :, h:h + 1].contiguous(), 0, where, at % page, torch.float64)[:, 0]
+            rows = q[i, 2 * h:2 * h + 2].double()
+            s = (k @ rows.t()) * scale                                                # [keys, 2]
+            lse[i, 2 * h:2 * h + 2] = torch.logsumexp(s, 0).float()
+            mine = lse[i, 2 * h:2 * h + 2].double()
+            w = torch.exp(s - mine)
+            off = 2.0 ** -24 * ((d + 8) * (k.abs() @ rows.abs().t()) * scale + 4 * (s.abs() + mine.abs()) + 8)
+            total = w.sum(1)
+            if previous:
+                total[:-1] += before[where[:-1], h, at[:-1] % page].double()
+            want[where, h, at % page] = total
+            bound[where, h, at % page] = (w * off).sum(1) + 2.0 ** -24 * 4 * total
+    out = torch.full_like(before, 9.0)
+    hip.attention_weights(q, cache, meta, lse, out, scale, window, previous=before if previous else None)
+    assert bool(((out.double() - want).abs() <= bound + 1e-30).all()), float(((out.double() - want).abs() / (bound + 1e-30)).max())
