@@ -103,10 +103,10 @@ FP4_WHOLE_KEYS = 160        # a step none of whose contexts is longer is not spl
 # their mean, the ordinary step, are not cut (160 of 4000 to 8200: 273 us).
 FP4_MOST_MEANS = 2
 # Items in blocks read unpacked pages, which takes a launch and writes and reads four times the bytes, but then every
-# product costs less than half: 5.6 against about 2.5 us a row tile and 32768 keys (48:8 heads of 128, one request).  16,
-# 64, 128 and 192 rows at 4096 keys take 48, 55, 59 and 63 us in blocks, 18, 32, 52 and 69 directly; 16, 32 and 128 at
-# 32768 keys 74, 82 and 175 against 47, 87 and 282; 32:8 heads of 64: 128 and 256 rows at 4096 keys 41 and 47 against 29
-# and 48, 32 and 96 at 32768 keys 53 and 70 against 38 and 88.  An item with at least so many tiles goes in blocks if
+# product costs less than half: 5.6 against about 2.5 us a row tile and 32768 keys (48:8 heads of 128, one request).  64,
+# 128 and 192 rows at 4096 keys take 51, 54 and 57 us in blocks, 32, 49 and 65 directly; 32 and 128 at 32768 keys 80 and 175
+# against 81 and 263; 512 at 16384 233 against 528; 32:8 heads of 64: 128 and 256 rows at 4096 keys 38 and 41 against 27
+# and 45, 96 at 32768 keys 66 against 87.  An item with at least so many tiles goes in blocks if
 # the step's items together have so many tiles beyond that, times the keys they read.
 FP4_BLOCK_TILES = 8
 FP4_BLOCK_WORK = 196608

@@ -45,3 +45,10 @@ def test_kept_work_lists_belong_to_their_lengths(guard, dtype, d):
 def test_joining_ranges(d, items):
     with Emulated() as hip:
         G.test_joining_ranges(hip, d, items)
+
+
+@pytest.mark.parametrize("case", [(6, 1, 128, 64, [300, 33, 1], [1, 1, 1], 0), (8, 2, 64, 32, [300, 90], [1, 3], 0), (4, 1, 256, 32, [200], [2], 0),
+                                  (6, 1, 128, 32, [200, 60], [1, 5], 50)])
+def test_probabilities_keep_what_their_rounding_leaves(case):
+    with Emulated() as hip:
+        G.test_probabilities_keep_what_their_rounding_leaves(hip, *case)

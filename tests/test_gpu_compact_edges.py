@@ -147,3 +147,19 @@ def test_weights_of_more_keys_than_one_round(hip, d, ctx, window, previous):
     out = torch.full_like(before, 9.0)
     hip.attention_weights(q, cache, meta, lse, out, scale, window, previous=before if previous else None)
     assert bool(((out.double() - want).abs() <= bound + 1e-30).all()), float(((out.double() - want).abs() / (bound + 1e-30)).max())
+
+
+@pytest.mark.parametrize("heads,kv,d,page,ctx,new,window", [
+    (6, 1, 128, 64, [300, 33, 1], [1, 1, 1], 0), (8, 2, 64, 32, [700, 90], [1, 3], 0), (4, 1, 256, 32, [300], [2], 0),
+    (6, 1, 128, 32, [200, 60], [1, 5], 50)])
+def test_probabilities_keep_what_their_rounding_leaves(hip, heads, kv, d, page, ctx, new, window):
+    """Attention read in 4 bits: a probability goes into the value product as two bfloat16, the second half a step of the
+    first at most, so that its own rounding is off by 2^-16 of the probability and the result's alone by 2^-8."""
+    meta, cache, q, of = C.attention_case("fp4", BF16, heads, kv, d, page, ctx, new, window)
+    out, lse = torch.empty(sum(new), heads * d, dtype=BF16).to(C.DEV), torch.empty(sum(new), heads).to(C.DEV)
+    hip.paged_attention(q.to(C.DEV), cache.to(C.DEV), meta, out, d ** -0.5, window, lse=lse)
+    want, _, spread, size = C.oracle.attention(q, of(0), of(1), ctx, new, d ** -0.5, window)
+    relative = 2.0 ** -24 * (2 * (d + 8) * size + max(ctx) + 64)
+    bound = spread * (relative[..., None] + 2.0 ** -16) + C.half_step(BF16) * want.abs()
+    error = (out.cpu().double().reshape(want.shape) - want).abs()
+    assert bool((error <= bound + 1e-30).all()), f"off by {float((error / (bound + 1e-30)).max()):.2f} of its bound"
