@@ -16,12 +16,13 @@
 // in base 2; a probability goes into the value product as two bfloat16, the second what the rounding of the first left
 // (2^-16 of it is lost), beside an unrounded running sum.  The result is then as near to 64 bits as one computed in float
 // and rounded once (a relative error of 0.00167 in the 2-norm, which is that rounding); with one bfloat16, as over the
-// engine's own cache, it is 0.00235.  The second product costs nothing where reading bounds the kernel (64 requests of
-// 8200 keys 92 us, 8 of 2100 12.0 instead of 11.7 us) and 3.5 of 47 us for 16 tokens on 32768 keys.
+// engine's own cache, it is 0.00235.  The second product costs 75 instead of 70 us for 4 requests of up to 131071 keys, 48
+// instead of 45 for 16 of 16384, 296 instead of 289 for 64 of 30000, 46 instead of 43 for 16 tokens of one on 32768 keys, and
+// nothing measurable for 8 of 2100 and at head size 256.
 //
 // Bound by reading the cache where there are keys enough, and by the latency of a wavefront's first loads else.  48:8
-// heads of 128: 4 requests of up to 131071 keys 67 us (6.1 TB/s) and 4.8 us for the merge of their ranges; 8 of up to
-// 2100 keys 9.0 + 3.7 us; one of 77 keys 6 us.
+// heads of 128: 4 requests of up to 131071 keys 71 us (5.8 TB/s) and 4.5 us for the merge of their ranges; 8 of up to
+// 2100 keys 8.8 + 2.8 us; one of 77 keys 6 us.
 //
 // head_dim 64, 128 or 256, page_size % 32 == 0 (a step of 32 keys lies in one page).
 #include "fp4.h"
@@ -352,24 +353,28 @@ paged_attention_fp4_kernel(const bf16_t* __restrict__ q, int64_t q_stride, const
         sum += p[j];
       }
       run_sum += sum;
-      uint4 pf, pr;      // as bfloat16, and what that rounding left, as bfloat16 again
+      uint4 pf;
       pf.x = floats_to_bf16x2_bits(p[0], p[1]);
       pf.y = floats_to_bf16x2_bits(p[2], p[3]);
       pf.z = floats_to_bf16x2_bits(p[4], p[5]);
       pf.w = floats_to_bf16x2_bits(p[6], p[7]);
-      pr.x = rest_of_bf16x2(p[0], p[1], pf.x);
-      pr.y = rest_of_bf16x2(p[2], p[3], pf.y);
-      pr.z = rest_of_bf16x2(p[4], p[5], pf.z);
-      pr.w = rest_of_bf16x2(p[6], p[7], pf.w);
+      auto add_values = [&](const uint4& weights) {
 #pragma unroll
-      for (int h = 0; h < P; ++h)
+        for (int h = 0; h < P; ++h)
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          o[h][w][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even[h][w], __builtin_bit_cast(bf16x8, pf), o[h][w][0], 0, 0, 0);
-          o[h][w][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd[h][w], __builtin_bit_cast(bf16x8, pf), o[h][w][1], 0, 0, 0);
-          o[h][w][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even[h][w], __builtin_bit_cast(bf16x8, pr), o[h][w][0], 0, 0, 0);
-          o[h][w][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd[h][w], __builtin_bit_cast(bf16x8, pr), o[h][w][1], 0, 0, 0);
-        }
+          for (int w = 0; w < 2; ++w) {
+            o[h][w][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even[h][w], __builtin_bit_cast(bf16x8, weights), o[h][w][0], 0, 0, 0);
+            o[h][w][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd[h][w], __builtin_bit_cast(bf16x8, weights), o[h][w][1], 0, 0, 0);
+          }
+      };
+      add_values(pf);
+      // The rest is made while those products run, and no product waits for the one before it.
+      uint4 rest;
+      rest.x = rest_of_bf16x2(p[0], p[1], pf.x);
+      rest.y = rest_of_bf16x2(p[2], p[3], pf.y);
+      rest.z = rest_of_bf16x2(p[4], p[5], pf.z);
+      rest.w = rest_of_bf16x2(p[6], p[7], pf.w);
+      add_values(rest);
     };
     // (The first loads stay in the order of their steps: mixed, the wait for the first step's in front of the loop, and
     // with it the one at the head of every round, would be a wait for all of them.)

@@ -88,9 +88,11 @@ def step_lengths(q_len, ctx_len) -> StepLengths:
 
 # A cache in 4 bits (the same heads; the kernel alone would be bound by reading at one wavefront per SIMD, and a few
 # too many, which run beside the others on some SIMDs, cost as much as twice as many everywhere).  4 requests of up to
-# 131071 keys take 70 us in at most 1024 ranges (6.1 TB/s in the kernel), 78 us in 2048, 85 us in 768; 16 x 16384 keys 44
-# against 49 us; but 64 requests x 8 heads are 512 tiles, whose ranges come in halves: 64 x 8200 keys 150 us unsplit,
-# 88 us in 2048.  A request of 77 keys takes 5.7 us whole and 7.4 in two ranges, 300 keys 9.5 us whole and 8.1 in five.
+# 131071 keys take 75 us in at most 1024 ranges, 79 us in 2048; one 34 against 39 us; 8 x 30000 keys 43 against 45; but 64
+# requests x 8 heads are 512 tiles, whose ranges come in halves: 64 x 8200 keys 150 us unsplit, 92 us in 1536 ranges.  (The
+# numbers of ranges that come of this are not always good ones: 32 x 30000 keys make 768, which leave a quarter of the SIMDs
+# idle, 64 x 30000 make 1536, two on one half of the SIMDs and one on the other, 4.6 TB/s where the four requests reach 5.8.)
+# A request of 77 keys takes 5.7 us whole and 7.4 in two ranges, 300 keys 9.5 us whole and 8.1 in five.
 # At head size 64 a step has half the bytes and one wavefront per SIMD is not enough (4 x 131071 keys, 32:8 heads: 50 us
 # in 1024 ranges, 43 in 2048).
 FP4_WAVES = 1024            # ranges wanted at head sizes from 128 on, while there are at least four to a tile;
