@@ -1,7 +1,9 @@
 // Into and out of the 4-bit cache (fp4.h):
 //   store:   the keys and values of a step's tokens, as they stand in the q | k | v rows, to their slots (where the
 //            norm and rotation kernel has not made the codes itself: no rotation and no norm, a norm per head,
-//            neighbouring pairs).  Bound by reading the rows: 8191 tokens of 8 + 8 heads of 128 take 18.7 us.
+//            neighbouring pairs).  8191 tokens of 8 + 8 heads of 128 take 18.7 us, 2.3 TB/s read and written, half of what a
+//            copy reaches: neighbouring lanes take neighbouring tokens, so that values are written side by side, but the
+//            16 bytes that the lanes of a load read lie whole rows apart.
 //   unpack:  whole pages to the engine's own page layout and type (what attention on many rows, in float32 and at
 //            head sizes without a kernel of its own reads).  Bound by writing: the 131 pages of 64 of such a step
 //            14 us (2.5 TB/s written), the 256 pages of a context of 16384 tokens 20 us (3.4).

@@ -680,7 +680,7 @@ class HipKernels:
         page_size, head_dim * 17 / 32]``, cache/layout.py): ``meta`` then needs its items, ``scale`` is positive, ``window`` not negative, and
         the call allocates what its longer way needs: partial results, and for the portions of prompts that it reads
         through unpacked pages a copy of those in ``q``'s type.  A key or value that is not a number reaches the rows that
-        see it and no others; over unpacked pages in bfloat16 all dims of theirs, else the value's groups of 32.
+        see it and no others; over unpacked pages in bfloat16 all dims of theirs, and their ``lse`` too, else the value's groups of 32.
         The first call on a meta leaves its lists in ``meta.work``, if it has one; they are for the lengths of that call."""
         tokens, heads, head_dim = q.shape
         kv_heads, page_size = cache.shape[2], cache.shape[3]
